@@ -161,6 +161,7 @@ def prepare(case, seed):
             # the tables need no K/V storage: a descriptor over one-row arenas
             s["arena"] = torch.empty((nblocks, 1, bs, 2), dtype=torch.float16, device=DEV)
             s["kv"] = rb.paged_kv_from_tensors(s["arena"], s["arena"], s["table"], s["cached"])
+            s["maps"] = rb.BatchTables.empty(case["seqs"], s["rows"], DEV)
     elif op == "append":
         lens = _lens(case, case["lens_lo"], case["lens_hi"])
         dt = DT[case["dtype"]]
@@ -236,7 +237,7 @@ def run(state):
 
 def _own_tables(s):
     import rustllm_b200 as rb
-    t = rb.batch_tables(s["kv"], s["new"], s["rows"], free_blocks=s["free"])
+    t = rb.batch_tables(s["kv"], s["new"], s["rows"], free_blocks=s["free"], out=s["maps"])
     return dict(table=s["table"], q_start=t.q_start, positions=t.positions, row_seq=t.row_seq,
                 slots=t.slots, info=t.info)
 
