@@ -389,6 +389,95 @@ int tmllm_gqa_prefill(const tmllm_paged_kv* kv, const void* q, const void* k_new
  * Synchronises with the device. */
 int tmllm_prefill_status(int32_t* status);
 
+/* ---------------------------------------------------------------------------------- */
+/* Packed prompts: requests of different lengths back to back                          */
+/* ---------------------------------------------------------------------------------- */
+
+/* New (the reference is batch 1).  Block tables and row maps of a packed batch, built on the
+ * GPU from request lengths: request s brings new_lens[s] tokens behind its kv->seq_lens[s]
+ * cached ones, its rows are q_start[s] .. q_start[s + 1] - 1 of the batch.
+ *   kv          block_table, seq_lens, num_seqs, max_blocks_per_seq, block_size, num_blocks
+ *               (the arenas are not touched and may be NULL)
+ *   new_lens    device int32 [num_seqs]; a negative length counts as 0
+ *   free_blocks device int32 [num_free] free block ids (num_free 0 with a non-NULL pointer: an
+ *               empty list), or NULL: every block is already in the table.  Request s takes need_s = ceil((len + new) / bs) - ceil(len / bs) ids in
+ *               request order, beginning at free_blocks[*free_start] (free_start: device int32,
+ *               NULL = 0), and they are written to its block_table entries from
+ *               ceil(len / bs) on.  The ids must be distinct and free; a table that
+ *               tmllm_cache_* manages keeps its own list, so pass NULL for it.
+ *   rows        capacity of the row arrays; rows beyond the batch get -1 in all three
+ * Outputs (device): q_start int32 [num_seqs + 1]; positions int32 [rows] (len + i); row_seq
+ * int32 [rows]; slots int64 [rows] (block * block_size + position % block_size, -1 without a
+ * block in [0, num_blocks)); info int32 [4] = {free list index behind the last id taken,
+ * rows of the batch, requests refused, rows beyond the capacity}.
+ * A request is refused - its rows get position and slot -1 and it takes no block - when its
+ * cached length is negative, its tokens pass max_blocks_per_seq * block_size, or it needs
+ * blocks and the needs of all requests up to it pass num_free.  Prefix sums are 64-bit and
+ * saturate in the int32 outputs.  The result depends on the arguments alone: calling again
+ * with the same arguments gives the same tables. */
+int tmllm_batch_tables(const tmllm_paged_kv* kv, const int32_t* new_lens,
+                       const int32_t* free_blocks, int32_t num_free, const int32_t* free_start,
+                       int64_t rows, int32_t* q_start, int32_t* positions, int32_t* row_seq,
+                       int64_t* slots, int32_t* info, tmllm_stream stream);
+
+/* Rotates packed rows at their positions (kernels/rope.metal:57-63, as tmllm_rope rounds) and
+ * scatters keys and values into the paged cache by slot (kernels/kv_cache_write.metal:13-18
+ * through the block table), in one pass.
+ *   kv        arenas, num_blocks, num_kv_heads, head_dim (even), block_size, dtype
+ *   q [rows, q_heads, head_dim], k, v [rows, num_kv_heads, head_dim] in the cache dtype; row
+ *             strides in elements (0 = packed), so a fused QKV projection is read in place
+ *   positions device int32 [rows]: a row with a negative position is padding and leaves every
+ *             output as it was; a position past rope_len is not rotated
+ *   slots     device int64 [rows]: block * block_size + offset; outside the arena nothing is
+ *             cached for the row.  Two rows with one slot leave it unspecified which row's
+ *             elements it holds.
+ *   rope_cos / rope_sin  [rope_len, head_dim / 2] F32, both NULL = no rotation
+ *   q_out     [rows, q_heads, head_dim] rotated queries (may be q itself, with its stride)
+ *   k_out     [rows, num_kv_heads, head_dim] rotated keys (may be k itself), or NULL */
+int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, const void* v,
+                      int64_t rows, int32_t q_heads, int64_t q_stride, int64_t kv_stride,
+                      const int32_t* positions, const int64_t* slots, const float* rope_cos,
+                      const float* rope_sin, int32_t rope_len, void* q_out, int64_t q_out_stride,
+                      void* k_out, int64_t k_out_stride, tmllm_stream stream);
+
+/* Replaces attention_core_encode (src/nn/attention.rs:216-247, start = 0) for a batch of whole
+ * prompts of different lengths, packed back to back: each query row attends the rows of its
+ * own sequence up to itself.
+ *   q [rows, q_heads, head_dim], k, v [rows, kv_heads, head_dim]: row strides in elements
+ *     (0 = packed); head_dim <= 256
+ *   q_start  device int32 [num_seqs + 1], non-decreasing first rows; sequences may be empty;
+ *     rows in front of q_start[0] and from q_start[num_seqs] on are neither read nor written
+ *   max_rows the longest sequence, or more (a bound for the launch)
+ *   scale    <= 0 means 1/sqrt(head_dim)
+ *   out      [rows, q_heads, head_dim] packed (dtype, or F32 if out_f32); may be q itself
+ *     (same type and stride), and must not overlap k or v
+ *   lse      [rows, q_heads] F32 natural-log sums of the scaled logits (NULL ok)
+ * Keys and values behind a row do not reach its result, whatever they hold.  A row whose
+ * logits are all -inf gives zeros and lse -inf.  F16 with head_dim a multiple of 8 up to 128
+ * and 16-byte aligned rows runs on the tensor cores, everything else on the CUDA cores. */
+int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, const void* k,
+                           const void* v, int64_t kv_stride, const int32_t* q_start,
+                           int32_t num_seqs, int64_t rows, int32_t max_rows, int32_t q_heads,
+                           int32_t kv_heads, int32_t head_dim, float scale, void* out,
+                           int32_t out_f32, float* lse, tmllm_stream stream);
+
+/* Replaces Linear::forward_encode (src/nn/linear.rs:105-170) with what follows it, for any
+ * number of rows: out = residual + act(x . W + bias), F16 tensors, F32 from the product to the
+ * one rounding of out.
+ *   x [rows, k], W [k, n] row-major; activation 0 none, 1 relu, 2 silu, 3 gelu (x Phi(x)),
+ *   4 swiglu: W is [k, 2n], gate then up columns, out = residual + silu(gate) * up;
+ *   bias F16 [n] (swiglu [2n]) or NULL; residual F16 [rows, n] or NULL (may be out itself).
+ * k and n multiples of 8, row strides multiples of 8 elements, x / W / residual / out 16-byte
+ * aligned. */
+int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                        int32_t activation, const void* residual, int64_t ldr, void* out,
+                        int64_t ldo, int32_t rows, int32_t k, int32_t n, tmllm_stream stream);
+
+/* Reads and clears the status of the bounded device-side waits in tmllm_prompt_attention and
+ * tmllm_prompt_linear on the current device: TMLLM_TIMEOUT when one expired since the last
+ * read (that call's outputs are undefined), else TMLLM_OK.  Synchronises with the device. */
+int tmllm_prompt_status(int32_t* status);
+
 /* Log-sum-exp merge of partial attention results (the combine step of a sequence split
  * across GPUs).  Part p's normalised output rows are at parts_o + p*o_stride ([rows,
  * head_dim] F32) and its log-sum-exp values at parts_lse + p*lse_stride ([rows] F32);

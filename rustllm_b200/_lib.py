@@ -191,6 +191,15 @@ _PROTOS = {
     "tmllm_gqa_prefill": (C.c_int, [C.POINTER(PagedKV), vp, vp, vp, vp, i32, i32, i32, vp, i32,
                                     C.POINTER(DecodeOpts), vp]),
     "tmllm_prefill_status": (C.c_int, [C.POINTER(i32)]),
+    "tmllm_batch_tables": (C.c_int, [C.POINTER(PagedKV), vp, vp, i32, vp, i64, vp, vp, vp, vp, vp,
+                                     vp]),
+    "tmllm_rope_append": (C.c_int, [C.POINTER(PagedKV), vp, vp, vp, i64, i32, i64, i64, vp, vp, vp,
+                                    vp, i32, vp, i64, vp, i64, vp]),
+    "tmllm_prompt_attention": (C.c_int, [C.c_int, vp, i64, vp, vp, i64, vp, i32, i64, i32, i32,
+                                         i32, i32, C.c_float, vp, i32, vp, vp]),
+    "tmllm_prompt_linear": (C.c_int, [vp, i64, vp, i64, vp, i32, vp, i64, vp, i64, i32, i32, i32,
+                                      vp]),
+    "tmllm_prompt_status": (C.c_int, [C.POINTER(i32)]),
     "tmllm_merge_lse": (C.c_int, [vp, vp, i32, i32, i32, i64, i64, vp, i32, vp, vp]),
     "tmllm_exchange_create": (C.c_int, [i32, i32, i32, i32, i32, C.POINTER(vp), vp]),
     "tmllm_exchange_connect": (C.c_int, [vp, vp]),

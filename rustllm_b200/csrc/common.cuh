@@ -47,6 +47,27 @@ int device_sm_count();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether two row-strided operands ([rows, width] at `stride`, elements of `es` bytes) share
+// memory.  Column ranges of one wider buffer (equal strides) do not, when they are disjoint.
+struct Rows {
+    const void* p;
+    int64_t stride, width;
+};
+inline bool overlaps(const Rows& a, const Rows& b, int64_t rows, size_t es) {
+    const int64_t a0 = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.p));
+    const int64_t b0 = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.p));
+    const int64_t e = static_cast<int64_t>(es);
+    if (a0 + ((rows - 1) * a.stride + a.width) * e <= b0 ||
+        b0 + ((rows - 1) * b.stride + b.width) * e <= a0)
+        return false;
+    if (a.stride == b.stride) {
+        const int64_t pitch = a.stride * e;
+        const int64_t m = ((b0 - a0) % pitch + pitch) % pitch;  // b's column behind a's
+        if (m >= a.width * e && m + b.width * e <= pitch) return false;
+    }
+    return true;
+}
+
 // Cross-GPU exchange of a sequence split (device-resident; see exchange.cu).  Every rank
 // owns one buffer of 8-byte cells {F32 value bits, step number}:
 //   recv_o   [2 parities][world][rows][head_dim]   normalised partial outputs

@@ -1,0 +1,369 @@
+// Projections of prompts (tmllm_prompt_linear): out = residual + act(x W + bias) for any number
+// of rows, the matrix product on the 5th-generation tensor cores and everything behind it in
+// its epilogue, so the product never makes a round trip through memory.
+//
+// F16 x [rows, k], W [k, n] row-major (nn/linear.rs:26-27), F32 accumulation and F32 all the
+// way through bias, activation (kernels/silu.metal:38-46 for SwiGLU) and residual, one
+// rounding to F16 at the store.
+#include <atomic>
+
+#include "common.cuh"
+#include "tc.cuh"
+
+namespace tmllm {
+namespace {
+
+constexpr int kM = 128;        // rows of an output tile (the tensor-memory lanes)
+constexpr int kK = 64;         // K columns per stage: one 128-byte swizzle row
+constexpr int kThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
+constexpr int kEpiThreads = 128;
+
+__device__ int g_linear_status;
+
+enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_SWIGLU = 4 };
+
+struct LinArgs {
+    const __half* bias;
+    const __half* residual;
+    int64_t ld_res;
+    int32_t rows, k, n, act;
+    int32_t m_tiles, n_tiles, tiles, group_m;
+};
+
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+// x Phi(x); through erfc, so the left tail keeps its relative accuracy
+__device__ __forceinline__ float gelu(float x) { return 0.5f * x * erfcf(-0.70710678f * x); }
+__device__ __forceinline__ float activate(float x, int act) {
+    if (act == ACT_RELU) return x > 0.f ? x : (x <= 0.f ? 0.f : x);  // NaN stays
+    if (act == ACT_SILU) return silu(x);
+    if (act == ACT_GELU) return gelu(x);
+    return x;
+}
+
+// BN: accumulator columns of a tile; with GATED half of them are gate and half up columns.
+template <int BN, bool GATED>
+struct LinCfg {
+    static constexpr int ON = GATED ? BN / 2 : BN;  // output columns of a tile
+    static constexpr int A_BYTES = kM * kK * 2;
+    static constexpr int B_BYTES = BN * kK * 2;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN == 256 ? 4 : 6;
+    static constexpr int OUT_BYTES = kM * 64 * 2;  // staging: 64 output columns
+    static constexpr int OFF_OUT = STAGES * STAGE;
+    static constexpr int OFF_BIAS = OFF_OUT + 2 * OUT_BYTES;
+    static constexpr int OFF_BAR = OFF_BIAS + 2 * BN * 2;  // bias as F16
+    static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment
+    static constexpr int TMEM_COLS = 2 * BN;           // two accumulators
+    static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
+};
+
+// Tile `t`: groups of group_m row tiles sweep the columns together, so a wave's A and W tiles
+// stay in L2.
+__device__ __forceinline__ void tile_of(const LinArgs& a, int t, int& m, int& n) {
+    const int per = a.group_m * a.n_tiles;
+    const int g = t / per, first = g * a.group_m;
+    const int gm = a.m_tiles - first < a.group_m ? a.m_tiles - first : a.group_m;
+    const int r = t - g * per;
+    m = first + r % gm;
+    n = r / gm;
+}
+
+template <int BN, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_linear_kernel(const __grid_constant__ CUtensorMap xmap,
+                         const __grid_constant__ CUtensorMap wmap,
+                         const __grid_constant__ CUtensorMap omap, const LinArgs a) {
+    using Cfg = LinCfg<BN, GATED>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t bars = sbase + Cfg::OFF_BAR;
+    auto full = [&](int i) { return bars + 8u * i; };
+    auto empty = [&](int i) { return bars + 8u * (Cfg::STAGES + i); };
+    auto acc_full = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + i); };
+    auto acc_empty = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + 2 + i); };
+    const uint32_t done = bars + 8u * (2 * Cfg::STAGES + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 8 * (2 * Cfg::STAGES + 5));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    if (tid == 0) {
+        for (int i = 0; i < Cfg::STAGES; ++i) {
+            mbar_init(full(i), 1);
+            mbar_init(empty(i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(acc_full(i), 1);
+            mbar_init(acc_empty(i), kEpiThreads);
+        }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(Cfg::TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int nk = (a.k + kK - 1) / kK;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int g = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+                int m, n;
+                tile_of(a, t, m, n);
+                for (int kb = 0; kb < nk; ++kb, ++g) {
+                    const int st = g % Cfg::STAGES, use = g / Cfg::STAGES;
+                    if (use > 0) {
+                        ok = mbar_wait_bounded(empty(st), (use - 1) & 1, abort_flag, &g_linear_status);
+                        if (!ok) break;
+                    }
+                    const uint32_t sa = sbase + st * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
+                    mbar_arrive_tx(full(st), Cfg::STAGE);
+                    tma_load_2d(sa, &xmap, kb * kK, m * kM, full(st));
+#pragma unroll
+                    for (int c = 0; c < BN / 64; ++c) {
+                        const int col = GATED ? (c < BN / 128 ? n * Cfg::ON + c * 64
+                                                              : a.n + n * Cfg::ON + (c - BN / 128) * 64)
+                                              : n * BN + c * 64;
+                        tma_load_2d(sb + c * (64 * kK * 2), &wmap, col, kb * kK, full(st));
+                    }
+                }
+            }
+            for (int i = g < Cfg::STAGES ? 0 : g - Cfg::STAGES; !ok && i < g; ++i)
+                mbar_drain(full(i % Cfg::STAGES), (i / Cfg::STAGES) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t IDESC = f16_idesc(kM, BN, true);
+            int g = 0, it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x, ++it) {
+                const int ab = it & 1;
+                if (it >= 2) {
+                    ok = mbar_wait_bounded(acc_empty(ab), ((it >> 1) - 1) & 1, abort_flag,
+                                           &g_linear_status);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                for (int kb = 0; kb < nk; ++kb, ++g) {
+                    const int st = g % Cfg::STAGES;
+                    ok = mbar_wait_bounded(full(st), (g / Cfg::STAGES) & 1, abort_flag,
+                                           &g_linear_status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t sa = sbase + st * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < kK / 16; ++kk)
+                        tc_mma(tmem + ab * BN, sw128_desc(sa + kk * 32, 16, 1024),
+                               sw128_desc(sb + kk * 2048, 64 * kK * 2, 1024), IDESC,
+                               kb > 0 || kk > 0);
+                    tc_commit(empty(st));
+                }
+                if (!ok) break;
+                tc_commit(acc_full(ab));
+            }
+            tc_commit(done);  // every product has completed before the CTA frees its memory
+            mbar_drain(done, 0);
+        }
+    } else {
+        const int et = tid - 64, quarter = warp & 3;
+        const int r = quarter * 32 + lane;  // this thread's row of the tile (its lane)
+        __half* bias_s = reinterpret_cast<__half*>(smem + Cfg::OFF_BIAS);
+        const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+        int it = 0, ob = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < a.tiles; t += gridDim.x, ++it) {
+            int m, n;
+            tile_of(a, t, m, n);
+            const int ab = it & 1;
+            __half* bias = bias_s + ab * BN;
+            if (a.bias) {
+                for (int c = et; c < BN; c += kEpiThreads) {
+                    const int col = GATED ? n * Cfg::ON + c % Cfg::ON : n * BN + c;
+                    const bool in = col < a.n;
+                    bias[c] = in ? a.bias[GATED && c >= Cfg::ON ? a.n + col : col] : __half(0.f);
+                }
+                named_barrier(1, kEpiThreads);
+            }
+            ok = mbar_wait_bounded(acc_full(ab), (it >> 1) & 1, abort_flag, &g_linear_status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const int64_t row = static_cast<int64_t>(m) * kM + r;
+            const bool live = row < a.rows;
+#pragma unroll 1
+            for (int c0 = 0; c0 < Cfg::ON; c0 += 64, ob ^= 1) {
+                const int col0 = n * Cfg::ON + c0;
+                if (col0 >= a.n) break;  // uniform: the rest of the tile is outside
+                // the staging buffer of two chunks ago has been read
+                if (et == 0) bulk_wait_read<1>();
+                named_barrier(1, kEpiThreads);
+                unsigned char* srow = smem + Cfg::OFF_OUT + ob * Cfg::OUT_BYTES + r * 128;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int cc = c0 + hf * 32;
+                    float y[32];
+                    tmem_ld32(tmem + ab * BN + cc + lane_base, y);
+                    if (a.bias) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] += __half2float(bias[cc + i]);
+                    }
+                    if (GATED) {
+                        float u[32];
+                        tmem_ld32(tmem + ab * BN + Cfg::ON + cc + lane_base, u);
+                        if (a.bias) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) u[i] += __half2float(bias[Cfg::ON + cc + i]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] = silu(y[i]) * u[i];
+                    } else if (a.act != ACT_NONE) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] = activate(y[i], a.act);
+                    }
+                    if (a.residual && live) {
+                        const __half* res = a.residual + row * a.ld_res + n * Cfg::ON + cc;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (n * Cfg::ON + cc + 8 * j >= a.n) break;
+                            const uint4 v = *reinterpret_cast<const uint4*>(res + 8 * j);
+                            float f[8];
+                            Chunk<__half>::unpack(v, f);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[8 * j + e] += f[e];
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<uint4*>(srow + (((hf * 4 + j) ^ (r & 7)) << 4)) =
+                            make_uint4(pack_half2(y[8 * j], y[8 * j + 1]),
+                                       pack_half2(y[8 * j + 2], y[8 * j + 3]),
+                                       pack_half2(y[8 * j + 4], y[8 * j + 5]),
+                                       pack_half2(y[8 * j + 6], y[8 * j + 7]));
+                }
+                fence_async_smem();
+                named_barrier(1, kEpiThreads);
+                if (et == 0) {
+                    tma_store_2d(&omap, col0, m * kM,
+                                 sbase + Cfg::OFF_OUT + ob * Cfg::OUT_BYTES);
+                    bulk_commit();
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(acc_empty(ab));
+        }
+        if (et == 0) bulk_wait<0>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(Cfg::TMEM_COLS)
+                     : "memory");
+    }
+}
+
+template <int BN, bool GATED>
+int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ldo,
+           LinArgs a, cudaStream_t s) {
+    using Cfg = LinCfg<BN, GATED>;
+    CUtensorMap xmap, wmap, omap;
+    if (int st = make_map(&xmap, x, a.k, a.rows, ldx * 2, kM)) return st;
+    if (int st = make_map(&wmap, w, GATED ? 2 * static_cast<int64_t>(a.n) : a.n, a.k, ldw * 2, kK))
+        return st;
+    if (int st = make_map(&omap, out, a.n, a.rows, ldo * 2, kM)) return st;
+    a.m_tiles = (a.rows + kM - 1) / kM;
+    a.n_tiles = (a.n + Cfg::ON - 1) / Cfg::ON;
+    int64_t tiles;
+    if (!mul_ok(a.m_tiles, a.n_tiles, &tiles) || tiles > INT32_MAX)
+        return fail(TMLLM_INVALID_SHAPE, "too many output tiles");
+    a.tiles = static_cast<int32_t>(tiles);
+    a.group_m = 16;
+    static std::atomic<uint64_t> opted{0};
+    int dev = 0;
+    TMLLM_CUDA_TRY(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? (1ull << dev) : 0;
+    if (!bit || !(opted.load(std::memory_order_relaxed) & bit)) {
+        TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_linear_kernel<BN, GATED>,
+                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            Cfg::SMEM));
+        opted.fetch_or(bit, std::memory_order_relaxed);
+    }
+    const int sms = device_sm_count();
+    const unsigned grid = static_cast<unsigned>(tiles < sms ? tiles : sms);
+    prompt_linear_kernel<BN, GATED><<<grid, kThreads, Cfg::SMEM, s>>>(xmap, wmap, omap, a);
+    TMLLM_LAUNCH_TRY();
+    return TMLLM_OK;
+}
+
+}  // namespace
+
+int take_linear_wait_status(int* out) {
+    int v = 0, zero = 0;
+    TMLLM_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_linear_status, sizeof(int)));
+    TMLLM_CUDA_TRY(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)));
+    *out = v;
+    return TMLLM_OK;
+}
+
+}  // namespace tmllm
+
+using namespace tmllm;
+
+extern "C" {
+
+int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                        int32_t activation, const void* residual, int64_t ldr, void* out,
+                        int64_t ldo, int32_t rows, int32_t k, int32_t n, tmllm_stream stream) {
+    clear_error();
+    if (rows < 0 || k <= 0 || n <= 0)
+        return fail(TMLLM_INVALID_SHAPE, "prompt_linear dimensions must be positive");
+    if (k % 8 || n % 8) return fail(TMLLM_INVALID_SHAPE, "prompt_linear needs k and n in multiples of 8");
+    if (activation < ACT_NONE || activation > ACT_SWIGLU)
+        return fail(TMLLM_INVALID_ARGUMENT, "unknown activation %d", activation);
+    const int64_t wide = activation == ACT_SWIGLU ? 2 * static_cast<int64_t>(n) : n;
+    if (rows > INT32_MAX - 1024 || k > INT32_MAX - 1024 || wide > INT32_MAX - 1024)
+        return fail(TMLLM_INVALID_SHAPE, "prompt_linear dimensions must fit 31 bits");
+    if (rows == 0) return TMLLM_OK;
+    if (!x || !w || !out) return fail(TMLLM_INVALID_ARGUMENT, "null tensor pointer");
+    int64_t span;
+    for (int64_t ld : {ldx, ldw, ldo, ldr})
+        if (ld % 8 || ld > (int64_t{1} << 38))  // the tensor maps' stride limit is 2^40 bytes
+            return fail(TMLLM_INVALID_SHAPE, "row strides must be multiples of 8 elements");
+    if (ldx < k || ldw < wide || ldo < n || (residual && ldr < n) || !mul_ok(rows, ldx, &span) ||
+        !mul_ok(rows, ldo, &span) || !mul_ok(k, ldw, &span) || (residual && !mul_ok(rows, ldr, &span)))
+        return fail(TMLLM_INVALID_SHAPE, "row strides must cover a row");
+    for (const void* p : {x, w, residual, static_cast<const void*>(out)})
+        if (!aligned16(p))
+            return fail(TMLLM_INVALID_ARGUMENT, "x, w, residual and out must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(bias) % 2)
+        return fail(TMLLM_INVALID_ARGUMENT, "bias must be aligned to its element size");
+    // tiles are stored while others are still read: out may be the residual itself only
+    if (overlaps({out, ldo, n}, {x, ldx, k}, rows, 2) ||
+        (residual && !(residual == out && ldr == ldo) &&
+         overlaps({out, ldo, n}, {residual, ldr, n}, rows, 2)))
+        return fail(TMLLM_INVALID_ARGUMENT, "out overlaps x, or the residual without being it");
+    LinArgs a{};
+    a.bias = static_cast<const __half*>(bias);
+    a.residual = static_cast<const __half*>(residual);
+    a.ld_res = ldr;
+    a.rows = rows;
+    a.k = k;
+    a.n = n;
+    a.act = activation;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (activation == ACT_SWIGLU) return launch<256, true>(x, ldx, w, ldw, out, ldo, a, s);
+    return launch<256, false>(x, ldx, w, ldw, out, ldo, a, s);
+}
+
+}  // extern "C"

@@ -7,6 +7,8 @@
 
 #include <cstdint>
 
+#include "tmllm.h"
+
 namespace tmllm {
 
 // Host: a 2-D tensor map over `rows` rows of `inner` elements, `row_bytes` apart, with
@@ -45,6 +47,54 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
         : "r"(bar), "r"(parity)
         : "memory");
     return ok != 0;
+}
+// Waits for the phase of parity `parity` of barrier `bar`, at most 2 s (a correct run waits
+// microseconds; the clock starts with this wait, so long kernels are no concern).  Gives up
+// (false) then, recording TMLLM_TIMEOUT in *status, or when another thread of the CTA did.
+__device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
+                                                  volatile int* abort_flag, int* status) {
+    unsigned long long t0 = 0;
+    for (uint32_t it = 0;; ++it) {
+        if (mbar_test(bar, parity)) return true;
+        if ((it & 63u) == 63u) {
+            if (*abort_flag) return false;
+            const unsigned long long now = global_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > 2000000000ull) {
+                *abort_flag = 1;
+                atomicExch(status, static_cast<int>(TMLLM_TIMEOUT));
+                return false;
+            }
+        }
+    }
+}
+// The same wait for what this thread itself has in flight (copies, products) before the CTA
+// gives its memory back, also after another thread gave up: bounded by tries alone (each
+// blocks for the hardware's own limit at most).
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < (1 << 14) && !mbar_test(bar, parity); ++i) {
+    }
+}
+// Stores a swizzled shared-memory box to a tensor map (elements outside the map's bounds are
+// dropped); completion through bulk groups.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// At most N of this thread's bulk groups still read their shared-memory source.
+template <int N> __device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+template <int N> __device__ __forceinline__ void bulk_wait() {
+    asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
                                             uint32_t bar) {
