@@ -30,7 +30,7 @@ struct PromptArgs {
     int64_t rows;
     int64_t q_stride, kv_stride, out_stride;
     int32_t num_seqs, max_rows, q_heads, kv_heads, group, head_dim, out_f32;
-    int32_t pairs;  // tensor-core form: two 128-row items a unit, or one
+    int32_t pairs;  // tensor-core form: a unit is 0 one item, 1 two heads, 2 two row tiles
     float scale_log2;
 };
 
@@ -195,103 +195,160 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 
 
 // ---- tensor-core form: F16, head size a multiple of 8 up to 128 -------------------------
-// An item is 128 query rows of one (sequence, query head).  The items of a (sequence, KV head)
-// are numbered row tile by row tile, heads of the group innermost; a unit is two neighbours, so
-// the K and V tiles it streams serve two items (two heads of the group over the same rows, or
-// two row tiles of one head when the group is one).  Per CTA:
-//   warps 0-3, 4-7  softmax of item 0 / 1, one thread per query row
+// Tiles are cut from the packed rows, not from the sequences: an item is 128 packed rows (whatever
+// sequences they belong to) of one query head, and a row sees the keys from its own sequence's
+// first row to itself.  So 500 prompts of one token are four row tiles, not 500.  Keys are tiled
+// on the same grid: the tile of the item's own rows is the last one it reads, the tile holding
+// the first row's sequence start the first one.
+// A unit is two items that stream the same K and V tiles: two heads of a KV group over the same
+// rows, or (odd groups) two neighbouring row tiles of one head.  Per CTA:
+//   warps 0-3, 4-7  softmax of item 0 / 1, one thread a query row
 //   warp 8          TMA producer: Q tiles, then K and V tiles through a ring
-//   warp 9          MMA issuer
-// S = Q K^T sits in tensor memory; its row is read to registers, exponentiated, and P written
-// back as F16 over the same columns, from where it is the A operand of O += P V (so only V
-// crosses shared memory for the second product).  While one item is exponentiated the tensor
-// cores work for the other one.
-//   tensor memory: S_i / P_i at [128 i, 128 i + 128), O_i at [256 + DP i, ...)
+//   warps 9, 10     MMA issuers of item 0 / 1
+// K and V arrive in tiles of 128 keys and are used in steps of 128 keys, or of 64 above head size
+// 64, where the accumulators leave less tensor memory.  S = Q K^T of a step sits in tensor memory;
+// its rows are read to registers (and the next step's S is computed over it), exponentiated, and P
+// is written to columns of its own as F16, from where it is the A operand of O += P V, so only V
+// crosses shared memory for the second product.
+//   tensor memory, KS keys a step: S_i at [KS i, + KS), P_i at [2 KS + KS / 2 i, + KS / 2), O_i at
+//   [512 - DP (2 - i), + DP)
 //
-// Masked places never reach a result: scores behind a row are replaced by -inf before the
-// maximum, and since 0 * inf is not 0, V's non-finite entries in a unit's diagonal tiles are
-// zeroed in shared memory before the product and added afterwards to the rows that see them.
+// Masked places never reach a result: scores that a row does not see are replaced by -inf before
+// the maximum, and since 0 * inf is not 0, the non-finite entries of every V tile that some row
+// of the unit does not see whole are zeroed in shared memory before the product and added
+// afterwards to the rows that see them ("scrubbed" tiles: the diagonal, the tile where the
+// sequence starts, all tiles of an item whose rows belong to several sequences).
 constexpr int kTile = 128;
-constexpr int kTcThreads = 384;  // warps 10 and 11 complete a warpgroup and idle
-constexpr int kMaxSeqs = 1024;    // sequences a launch schedules
-constexpr int kMaxLevels = 4096;  // row tiles of a sequence: prompts of up to 524,288 rows
+constexpr int kTcThreads = 384;  // warp 11 completes a warpgroup and idles
+constexpr int kWindow = 2048;    // row tiles a launch schedules (262,144 packed rows)
 
 template <int DP>
 struct AttCfg {
     static constexpr int BLK = 16384;          // 64 columns x 128 rows, swizzled
     static constexpr int TILE = DP / 64 * BLK; // Q, K or V tile
     static constexpr int QBUF = DP == 64 ? 2 : 1;
-    static constexpr int STAGES = DP == 64 ? 6 : 4;
+    static constexpr int STAGES = DP == 64 ? 8 : 4;
     static constexpr int OFF_KV = 2 * QBUF * TILE;
-    static constexpr int OFF_BASE = OFF_KV + STAGES * TILE;    // int32 units before each level
-    static constexpr int OFF_ORDER = OFF_BASE + kMaxLevels * 4;  // uint16 sequences, longest first
-    static constexpr int OFF_TILES = OFF_ORDER + kMaxSeqs * 2;  // int32 their row tiles
-    static constexpr int OFF_BAR = OFF_TILES + kMaxSeqs * 4;
+    static constexpr int OFF_SEQ = OFF_KV + STAGES * TILE;      // int32 sequence of a tile's first row
+    static constexpr int OFF_HIST = OFF_SEQ + kWindow * 4;      // int32 row tiles of each cost
+    static constexpr int OFF_LIST = OFF_HIST + kWindow * 4;     // uint16 row tiles, longest first
+    static constexpr int OFF_BAR = OFF_LIST + kWindow * 2;
+    static constexpr int KS = DP == 64 ? 128 : 64;  // keys of a step
+    static constexpr int SPT = 128 / KS;            // steps of a key tile
+    static_assert(3 * KS + 2 * DP <= 512, "tensor memory");
     static constexpr int SMEM = OFF_BAR + 512 + 1024;  // + alignment
     static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 };
 
-// Barriers: QF/QE Q tile full / empty, KF/KE ring full / empty, S scores ready, P probabilities
-// written, O product done, E accumulator read, VR diagonal V tile loaded, SB scrubbed, DONE all
-// products.  VR and SB exist twice, for a unit's first and second diagonal tile ("events"): every
-// unit passes the first one, and both softmax groups take part in each, so no thread ever falls
-// more than a phase behind a barrier that it waits on.
+// Barriers: QF/QE Q tile full / empty, KF/KE ring full / empty; of each item: S scores ready, F
+// scores read, P probabilities written, O product done, E accumulator read; VR a V tile to scrub
+// has landed, SB it is scrubbed, DONE all products.  Both softmax groups and both MMA warps take
+// part in every scrub (every unit has one, its diagonal) and both MMA warps give back every K and
+// V tile, whether their item uses it or not, so no thread ever falls more than a phase behind a
+// barrier that it waits on.
 template <int DP>
 struct AttBar {
     using Cfg = AttCfg<DP>;
     static constexpr int QF = 0, QE = QF + 2 * Cfg::QBUF, KF = QE + 2 * Cfg::QBUF,
-                         KE = KF + Cfg::STAGES, S = KE + Cfg::STAGES, P = S + 2, O = P + 2,
-                         E = O + 2, VR = E + 2, SB = VR + 2, DONE = SB + 2, COUNT = DONE + 1;
+                         KE = KF + Cfg::STAGES, S = KE + Cfg::STAGES, F = S + 2, P = F + 2,
+                         O = P + 2, E = O + 2, VR = E + 2, SB = VR + 1, DONE = SB + 1,
+                         COUNT = DONE + 1;
     static_assert(COUNT * 8 + 64 <= 512, "barrier area");
 };
 
+// Last sequence whose first row is <= row, among [lo, num_seqs).
+__device__ __forceinline__ int seq_at(const PromptArgs& a, int row, int lo) {
+    int hi = a.num_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (__ldg(a.q_start + mid) <= row) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
 struct AttUnit {
-    int64_t row0;
-    int n;           // rows of the sequence
-    int kvh;
-    int head[2], q_lo[2];
-    int nt[2];       // key tiles of each item; 0: no such item
+    int kvh, jlo, jhi;         // key tiles the unit streams
+    int head[2], tile[2];      // query head and row tile of each item
+    int lo[2], hi[2];          // its steps (lo > hi: no such item)
+    int seq[2];                // sequence of the item's first row
+    bool several[2];           // its rows belong to more than one
+    bool any_several;
+    int first;                 // first visible key of the unit's first row
+    __device__ __forceinline__ bool on(int i) const { return lo[i] <= hi[i]; }
+    // the same values in every lane, and known to be
+    __device__ __forceinline__ void make_uniform() {
+        auto bc = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+        kvh = bc(kvh), jlo = bc(jlo), jhi = bc(jhi), first = bc(first);
+        any_several = bc(any_several);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            head[i] = bc(head[i]), tile[i] = bc(tile[i]), lo[i] = bc(lo[i]), hi[i] = bc(hi[i]);
+            seq[i] = bc(seq[i]), several[i] = bc(several[i]);
+        }
+    }
+    // some row of the unit does not see key tile j whole
+    __device__ __forceinline__ bool ragged(int j) const {
+        return any_several || j == tile[0] || j == tile[1] || j * kTile < first;
+    }
 };
 
-// The work list every role of every CTA walks in the same order: longest key range first, dealt
-// to the CTAs in a snake, so their sums come out alike.  A level is a row tile index; levels
-// are visited from the last to the first, the sequences that reach one in order of length.
+// The work list every role of every CTA walks in the same order: row tiles with the longest key
+// range first, heads innermost (they share K and V in L2), dealt to the CTAs in a snake so their
+// sums come out alike.
 struct AttSched {
-    const int32_t* base;    // units in the levels above
-    const uint16_t* order;
-    int level, levels, total, k;
+    const int32_t* tile_seq;
+    const uint16_t* list;
+    int row_lo, row_hi;        // live rows
+    int tile0, per, total, k;  // window's first tile, units of a list entry
 
+    template <int KS>
     __device__ __forceinline__ bool next(const PromptArgs& a, AttUnit& u) {
-        for (;;) {
-            const int G = gridDim.x;
-            const int64_t at = (k & 1) ? static_cast<int64_t>(k + 1) * G - 1 - blockIdx.x
-                                       : static_cast<int64_t>(k) * G + blockIdx.x;
-            if (static_cast<int64_t>(k) * G >= total) return false;
+        const int G = gridDim.x;
+        int idx;
+        do {
+            const int64_t base = static_cast<int64_t>(k) * G;
+            if (base >= total) return false;
+            const int64_t at = (k & 1) ? base + G - 1 - blockIdx.x : base + blockIdx.x;
             ++k;
-            if (at >= total) continue;
-            const int idx = static_cast<int>(at);
-            while (level > 0 && idx >= base[level - 1]) --level;
-            const int g = a.group, t = level;
-            const int p0 = a.pairs ? (t * g + 1) / 2 : t * g;
-            const int np = a.pairs ? ((t + 1) * g + 1) / 2 - p0 : g;
-            int r = idx - base[t];
-            const int p = p0 + r % np;
-            r /= np;
-            u.kvh = r % a.kv_heads;
-            const int s = order[r / a.kv_heads];
-            u.n = seq_rows(a, s, &u.row0);
-            const int tiles = (u.n + kTile - 1) / kTile;
+            idx = at < total ? static_cast<int>(at) : -1;
+        } while (idx < 0);
+        const int rank = idx / per;
+        int rem = idx - rank * per;
+        const int np = per / a.kv_heads;
+        u.kvh = rem / np;
+        rem -= u.kvh * np;
+        u.any_several = false;
+        const int st = list[rank];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int item = a.pairs ? 2 * p + i : p;
-                const int tile = item / g;
-                const bool in = (i == 0 || a.pairs) && tile < tiles;
-                u.head[i] = u.kvh * g + item % g;
-                u.q_lo[i] = tile * kTile;
-                u.nt[i] = in ? tile + 1 : 0;
-            }
-            return true;
+        for (int i = 0; i < 2; ++i) {
+            int tile = st, g = rem;
+            bool in = true;
+            if (a.pairs == 1) g = 2 * rem + i;     // two heads of the group
+            else if (a.pairs == 2) tile = 2 * st + i;  // two row tiles of one head
+            else in = i == 0;
+            const int r0 = (tile0 + tile) * kTile;
+            in = in && r0 < row_hi && r0 + kTile > row_lo;
+            u.head[i] = u.kvh * a.group + g;
+            u.tile[i] = tile0 + tile;
+            u.lo[i] = 1;
+            u.hi[i] = 0;
+            u.several[i] = false;
+            u.seq[i] = 0;
+            if (!in) continue;
+            const int s = tile_seq[tile];
+            const int end = r0 + kTile < row_hi ? r0 + kTile : row_hi;
+            u.seq[i] = s;
+            u.several[i] = __ldg(a.q_start + s + 1) < end;
+            u.any_several |= u.several[i];
+            const int first = max(__ldg(a.q_start + s), 0);
+            u.lo[i] = first / KS;
+            u.hi[i] = (end - 1) / KS;
+            if (i == 0 || !u.on(0)) u.first = first;
         }
+        u.jlo = (u.on(0) ? u.lo[0] : u.lo[1]) / (kTile / KS);
+        u.jhi = (u.on(1) ? u.hi[1] : u.hi[0]) / (kTile / KS);
+        return true;
     }
 };
 
@@ -300,35 +357,41 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
+}
 __device__ __forceinline__ bool odd_half(uint32_t bits) { return (bits & 0x7C00u) == 0x7C00u; }
 
 template <int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap qmap,
                      const __grid_constant__ CUtensorMap kmap,
-                     const __grid_constant__ CUtensorMap vmap, const PromptArgs a) {
+                     const __grid_constant__ CUtensorMap vmap, const PromptArgs a, int tile0) {
     using Cfg = AttCfg<DP>;
     using B = AttBar<DP>;
+    constexpr int KS = Cfg::KS, SPT = Cfg::SPT;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform for the compiler too
     const uint32_t bars = sbase + Cfg::OFF_BAR;
     auto bar = [&](int i) { return bars + 8u * static_cast<uint32_t>(i); };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + B::COUNT * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* odd_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [parity][event]
-    int* scan = reinterpret_cast<int*>(tmem_slot + 6);  // one total
+    volatile int* odd_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [unit parity]
     constexpr unsigned FULL = 0xffffffffu;
 
     if (tid == 0) {
         for (int i = 0; i < B::COUNT; ++i) {
-            const bool softmax = i >= B::P && i < B::P + 2;
-            const bool epilogue = i >= B::E && i < B::E + 2;
-            mbar_init(bar(i), i >= B::SB && i < B::SB + 2 ? 256u : (softmax || epilogue) ? 128u : 1u);
+            const bool group = i >= B::F && i < B::E + 2 && !(i >= B::O && i < B::O + 2);
+            const bool both = i == B::VR || i == B::DONE || (i >= B::KE && i < B::KE + Cfg::STAGES);
+            mbar_init(bar(i), i == B::SB ? 256u : group ? 128u : both ? 2u : 1u);
         }
         *abort_flag = 0;
-        for (int i = 0; i < 4; ++i) odd_flag[i] = 0;
+        odd_flag[0] = odd_flag[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) {
@@ -339,67 +402,83 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // ---- the work list
-    int32_t* base = reinterpret_cast<int32_t*>(smem + Cfg::OFF_BASE);
-    uint16_t* order = reinterpret_cast<uint16_t*>(smem + Cfg::OFF_ORDER);
-    int32_t* tiles = reinterpret_cast<int32_t*>(smem + Cfg::OFF_TILES);
-    int32_t* raw = base;  // unsorted row tiles, until the levels are written
-    for (int s = tid; s < a.num_seqs; s += kTcThreads) {
-        int64_t r0;
-        raw[s] = (seq_rows(a, s, &r0) + kTile - 1) / kTile;
-    }
-    __syncthreads();
-    for (int s = tid; s < a.num_seqs; s += kTcThreads) {
-        const int mine = raw[s];
-        int rank = 0;  // longer sequences, and equally long ones in front
-        for (int o = 0; o < a.num_seqs; ++o) rank += raw[o] > mine || (raw[o] == mine && o < s);
-        order[rank] = static_cast<uint16_t>(s);
-        tiles[rank] = mine;
+    int32_t* tile_seq = reinterpret_cast<int32_t*>(smem + Cfg::OFF_SEQ);
+    int32_t* hist = reinterpret_cast<int32_t*>(smem + Cfg::OFF_HIST);
+    uint16_t* list = reinterpret_cast<uint16_t*>(smem + Cfg::OFF_LIST);
+    AttSched sched{tile_seq, list, 0, 0, tile0, 0, 0, 0};
+    {
+        const int q0 = __ldg(a.q_start), q1 = __ldg(a.q_start + a.num_seqs);
+        sched.row_lo = q0 > 0 ? q0 : 0;
+        sched.row_hi = q1 < a.rows ? q1 : static_cast<int>(a.rows);
+        const int span = a.pairs == 2 ? 2 : 1;  // row tiles of a list entry
+        // live tiles of the window, relative to its first
+        int ta = sched.row_lo / kTile - tile0, tb = (sched.row_hi + kTile - 1) / kTile - tile0;
+        ta = ta > 0 ? ta : 0;
+        tb = tb < kWindow ? tb : kWindow;
+        const int ea = ta / span, eb = (tb + span - 1) / span;
+        const int count = sched.row_hi > sched.row_lo && eb > ea ? eb - ea : 0;
+        sched.per = a.kv_heads * (a.pairs == 1 ? a.group / 2 : a.group);
+        sched.total = count * sched.per;
+        const bool sorted = sched.total > static_cast<int>(gridDim.x);
+        for (int i = tid; i < kWindow; i += kTcThreads) hist[i] = 0;
+        auto cost_of = [&](int e) {
+            const int t0 = max(e * span, ta), t1 = min(e * span + span, tb) - 1;
+            const int c = tile0 + t1 - max(__ldg(a.q_start + tile_seq[t0]), 0) / kTile;
+            return c < kWindow ? c : kWindow - 1;
+        };
+        for (int t = ta + tid; t < tb; t += kTcThreads) {
+            const int row = (tile0 + t) * kTile;
+            tile_seq[t] = seq_at(a, row > sched.row_lo ? row : sched.row_lo, 0);
+        }
+        __syncthreads();
+        if (!sorted) {
+            for (int i = tid; i < count; i += kTcThreads) list[i] = static_cast<uint16_t>(ea + i);
+        } else {
+            for (int i = tid; i < count; i += kTcThreads) atomicAdd(hist + cost_of(ea + i), 1);
+            __syncthreads();
+            if (warp == 0) {
+                int above = 0;  // entries of a higher cost
+                const int most = tile0 + tb < kWindow ? tile0 + tb : kWindow - 1;
+                for (int c0 = most; c0 >= 0; c0 -= 32) {
+                    const int c = c0 - lane, own = c >= 0 ? hist[c] : 0;
+                    int sum = own;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int x = __shfl_up_sync(FULL, sum, o);
+                        if (lane >= o) sum += x;
+                    }
+                    if (c >= 0) hist[c] = above + sum - own;
+                    above += __shfl_sync(FULL, sum, 31);
+                }
+                __syncwarp();
+                // in order within a cost, so every CTA has the same list
+                for (int i0 = 0; i0 < count; i0 += 32) {
+                    const int i = i0 + lane;
+                    const int c = i < count ? cost_of(ea + i) : -1;
+                    const unsigned same = __match_any_sync(FULL, c);
+                    const int before = __popc(same & ((1u << lane) - 1u));
+                    const int at = c >= 0 ? hist[c] : 0;
+                    __syncwarp();
+                    if (c >= 0) {
+                        list[at + before] = static_cast<uint16_t>(ea + i);
+                        if (before == 0) hist[c] = at + __popc(same);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    AttSched sched{base, order, 0, tiles[0], 0, 0};
-    {
-        // units of level t: the sequences with more than t tiles x KV heads x pairs starting in
-        // it; then the sum over the levels above, one warp scanning downwards
-        for (int t = tid; t < sched.levels; t += kTcThreads) {
-            int lo = 0, hi = a.num_seqs;  // first rank with at most t tiles
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (tiles[mid] > t) lo = mid + 1;
-                else hi = mid;
-            }
-            const int np = a.pairs ? ((t + 1) * a.group + 1) / 2 - (t * a.group + 1) / 2 : a.group;
-            base[t] = lo * a.kv_heads * np;
-        }
-        __syncthreads();
-        if (warp == 0) {
-            int above = 0;
-            for (int t0 = sched.levels - 1; t0 >= 0; t0 -= 32) {
-                const int t = t0 - lane;
-                const int own = t >= 0 ? base[t] : 0;
-                int sum = own;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int x = __shfl_up_sync(FULL, sum, o);
-                    if (lane >= o) sum += x;
-                }
-                if (t >= 0) base[t] = above + sum - own;
-                above += __shfl_sync(FULL, sum, 31);
-            }
-            if (lane == 0) *scan = above;
-        }
-        __syncthreads();
-        sched.total = *scan;
-        sched.level = sched.levels > 0 ? sched.levels - 1 : 0;
-    }
     const uint32_t tmem = *tmem_slot;
-    auto tmem_s = [&](int i) { return tmem + 128u * i; };
-    auto tmem_o = [&](int i) { return tmem + 256u + static_cast<uint32_t>(DP) * i; };
+    auto tmem_s = [&](int i) { return tmem + static_cast<uint32_t>(KS * i); };
+    auto tmem_p = [&](int i) { return tmem + static_cast<uint32_t>(2 * KS + KS / 2 * i); };
+    auto tmem_o = [&](int i) { return tmem + static_cast<uint32_t>(512 - DP * (2 - i)); };
     auto wait = [&](int b, uint32_t parity) {
         return mbar_wait_bounded(bar(b), parity & 1u, abort_flag, &g_attention_status);
     };
-    AttUnit u;
+    AttUnit u{};
 
     // A row of S takes 128 registers: the softmax groups get 200 each out of the launch's 168,
     // the others' warpgroup 96 (2 x 200 + 96 <= 3 x 168 in each quarter of the SM).
@@ -409,108 +488,134 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int w = warp >> 2, r = tid & 127;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem_s(w) + lane_base, to = tmem_o(w) + lane_base;
-        int step = 0, ring0 = 0, unit = 0, second = 0;
-        bool ok = true;
-        // Non-finite entries of the V tile of key tile j become zeros (and raise the flag); all
-        // 256 softmax threads share the tile.
-        auto scrub = [&](int j, int event) {
-            const int st = (ring0 + 2 * j + 1) % Cfg::STAGES;
-            ok = wait(B::VR + event, event ? second++ : unit);
-            ok = __all_sync(FULL, ok);
-            if (!ok) return;
-            unsigned char* v = smem + Cfg::OFF_KV + st * Cfg::TILE;
-            uint4 x[DP / 16];
+        const uint32_t tp = tmem_p(w) + lane_base;
+        const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
+        int step = 0, ring0 = 0, unit = 0, events = 0;
+        auto await = [&](int b, int phase) {
+            mbar_wait_uniform(bar(b), phase & 1, abort_addr, &g_attention_status);
+        };
+        // Non-finite entries of the V tile of key tile j become zeros (and raise the unit's
+        // flag); all 256 softmax threads share the tile.
+        auto scrub = [&](int j) {
+            const int st = (ring0 + 2 * (j - u.jlo) + 1) % Cfg::STAGES;
+            await(B::VR, events++);
+            unsigned char* v = smem + Cfg::OFF_KV + st * Cfg::TILE + tid * 16;
             __half2 probe = __floats2half2_rn(0.f, 0.f);
             const __half2 zero = probe;
-            const int nb = (a.head_dim + 63) / 64;  // boxes behind it were never loaded
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) {
-                if (c * 4096 < nb * Cfg::BLK) {
-                    x[c] = *reinterpret_cast<const uint4*>(v + (tid + 256 * c) * 16);
-                    const __half2* h = reinterpret_cast<const __half2*>(&x[c]);
+                const uint4 x = *reinterpret_cast<const uint4*>(v + 4096 * c);
+                const __half2* h = reinterpret_cast<const __half2*>(&x);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) probe = __hfma2(h[e], zero, probe);  // 0 or NaN
-                }
+                for (int e = 0; e < 4; ++e) probe = __hfma2(h[e], zero, probe);  // 0 or NaN
             }
             if (!(__low2float(probe) == 0.f && __high2float(probe) == 0.f)) {
-                odd_flag[(unit & 1) * 2 + event] = unit + 1;
-                for (int c = 0; c * 4096 < nb * Cfg::BLK; ++c) {
-                    __half* p = reinterpret_cast<__half*>(v + (tid + 256 * c) * 16);
+                odd_flag[unit & 1] = unit + 1;
+                for (int c = 0; c < DP / 16; ++c) {
+                    __half* p = reinterpret_cast<__half*>(v + 4096 * c);
                     for (int e = 0; e < 8; ++e)
                         if (odd_half(__half_as_ushort(p[e]))) p[e] = __float2half_rn(0.f);
                 }
             }
+            __syncwarp();
             fence_async_smem();
-            mbar_arrive(bar(B::SB + event));
+            mbar_arrive(bar(B::SB));
         };
-        for (; ok && sched.next(a, u); ++unit) {
-            const int nt = u.nt[w];
-            const int jd0 = u.nt[0] - 1, jd1 = u.nt[1] - 1;
-            const int rows = u.n - u.q_lo[w] < kTile ? u.n - u.q_lo[w] : kTile;
-            const int qpos = u.q_lo[w] + r;  // keys 0 .. qpos are visible
+        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+        for (; sched.template next<Cfg::KS>(a, u) && !*abort_flag; ++unit) {
+            const int lo = w ? u.lo[1] : u.lo[0], hi = w ? u.hi[1] : u.hi[0];
+            const int tile = w ? u.tile[1] : u.tile[0], head = w ? u.head[1] : u.head[0];
+            const int row = tile * kTile + r;  // keys `first` .. row are visible
+            const bool on = lo <= hi;
+            const bool live = on && row >= sched.row_lo && row < sched.row_hi;
+            int first = INT32_MAX;
+            if (live) {
+                const int s0 = w ? u.seq[1] : u.seq[0];
+                const bool several = w ? u.several[1] : u.several[0];
+                first = max(__ldg(a.q_start + (several ? seq_at(a, row, s0) : s0)), 0);
+            }
             float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < nt; ++j, ++step) {
-                if (j == jd0 || j == jd1) {
-                    scrub(j, j == jd0 ? 0 : 1);
-                    if (!ok) break;
-                }
-                ok = wait(B::S + w, step);
-                ok = __all_sync(FULL, ok);
-                if (!ok) break;
+            for (int n = u.jlo * SPT; n <= u.jhi * SPT + SPT - 1; ++n) {
+                const bool ragged = u.ragged(n / SPT);
+                if (ragged && n % SPT == 0) scrub(n / SPT);
+                if (n < lo || n > hi) continue;
+                await(B::S + w, step);
                 tc_fence_after();
-                float v[128];
-                tmem_ld4x32(ts, v);
-                const int lim = qpos - j * kTile;  // columns 0 .. lim are visible
-                const bool diag = j == nt - 1;
-                if (diag) {
+                float v[KS];
+                tmem_ld_row(ts, v);
+                tc_fence_before();
+                mbar_arrive(bar(B::F + w));
+                int dark_lo = 0, dark_hi = KS - 1;  // columns some row of the warp sees
+                if (ragged) {
+                    // columns c_lo .. c_hi of this row are visible
+                    const int c_lo = live ? first - n * KS : KS;
+                    const int c_hi = live ? row - n * KS : -1;
+                    dark_lo = __reduce_min_sync(FULL, c_lo);
+                    dark_hi = __reduce_max_sync(FULL, c_hi);
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) v[i] = i <= lim ? v[i] : -INFINITY;
+                    for (int i = 0; i < KS; ++i)
+                        v[i] = (i >= c_lo && i <= c_hi) ? v[i] : -INFINITY;
                 }
-                float mx = -INFINITY;
+                auto row_max = [&]() {
+                    float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                for (int i = 0; i < 128; ++i) mx = fmaxf(mx, v[i]);
-                const float mt = mx * a.scale_log2;
-                // O and l are rescaled only when the maximum grew by more than 2^8: P stays
-                // below 2^8 and 1 / l makes up for it.  -inf (nothing visible yet) always is.
+                    for (int i = 4; i < KS - 4; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], v[i + e], v[i + 4 + e]);
+                    return fmaxf(max3(mx[0], mx[1], fmaxf(v[KS - 4], v[KS - 3])),
+                                 max3(mx[2], mx[3], fmaxf(v[KS - 2], v[KS - 1]))) *
+                           a.scale_log2;
+                };
+                // P is taken relative to the running maximum m of the steps before, which is
+                // known at once, and this step's own maximum is found meanwhile.  Only when it
+                // exceeds m by more than 2^8 does m follow (P is computed again, O and l are
+                // rescaled); else P stays below 2^8 and 1 / l makes up for it.
+                const bool begin = n == lo;
+                if (begin) m = row_max();
                 float alpha = 1.f;
-                const bool grow = j == 0 || mt > m + 8.f;
-                const bool need = j > 0 && grow;
-                if (grow) {
-                    if (need) {
-                        alpha = m == -INFINITY ? 0.f : exp2_approx(m - mt);
-                        l *= alpha;
-                    }
-                    m = mt;
+                bool grown = false;  // of some row of the warp
+                float2 l2[2];
+                if (!begin) {  // the product before has read P
+                    await(B::O + w, step - 1);
+                    tc_fence_after();
                 }
-                const float sub = m == -INFINITY ? 0.f : -m;
-                const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-                const float2 sub2 = make_float2(sub, sub);
-                float2 l2 = make_float2(0.f, 0.f);
+                for (;;) {
+                    // -inf (nothing visible yet): exp2(-inf - 0) = 0
+                    const float sub = m == -INFINITY ? 0.f : -m;
+                    const float2 sub2 = make_float2(sub, sub);
+                    l2[0] = l2[1] = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t pk[32];
+                    for (int c = 0; c < KS / 32; ++c) {
+                        uint32_t pk[16];
+                        // 32 columns no row of the warp sees: zeros without exponentials
+                        if (c * 32 <= dark_hi && c * 32 + 31 >= dark_lo) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        // 32 columns no row of the warp can see: zeros without exponentials
-                        const int c0 = hf * 64 + c * 32;
-                        const bool dark = diag && c0 > (warp & 3) * 32 + 31;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int i = c0 + 2 * e;
-                            uint32_t bits = 0u;
-                            if (!dark) {
+                            for (int e = 0; e < 16; ++e) {
+                                const int i = c * 32 + 2 * e;
                                 const float2 x = __ffma2_rn(make_float2(v[i], v[i + 1]), sc2, sub2);
                                 const float2 p = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-                                l2 = __fadd2_rn(l2, p);
-                                bits = pack_half2(p.x, p.y);
+                                l2[e & 1] = __fadd2_rn(l2[e & 1], p);
+                                pk[e] = pack_half2(p.x, p.y);
                             }
-                            pk[c * 16 + e] = bits;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) pk[e] = 0u;
                         }
+                        tmem_st16_bits(tp + 16 * c, pk);
                     }
-                    tmem_st32_bits(ts + hf * 32, pk);
+                    if (begin) break;
+                    const float mt = row_max();
+                    const bool grow = mt > m + 8.f;
+                    if (!__any_sync(FULL, grow)) break;
+                    grown = true;
+                    if (grow) {
+                        alpha = m == -INFINITY ? 0.f : exp2_approx(m - mt);
+                        l *= alpha;
+                        m = mt;
+                    }
                 }
-                l += l2.x + l2.y;
-                if (__any_sync(FULL, need)) {  // the product before is done: S of this step follows it
+                l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+                if (grown) {  // O holds the products before this step
 #pragma unroll 1
                     for (int c = 0; c < DP / 32; ++c) {
                         float o[32];
@@ -523,49 +628,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(bar(B::P + w));
+                ++step;
             }
-            if (!ok) break;
-            if (w == 0 && jd1 > jd0) scrub(jd1, 1);
-            if (w == 1 && nt == 0) scrub(jd0, 0);
-            if (!ok) break;
-            ring0 += 2 * (u.nt[1] > u.nt[0] ? u.nt[1] : u.nt[0]);
-            if (nt == 0) continue;
+            ring0 += 2 * (u.jhi - u.jlo + 1);
+            if (!on) continue;
             // ---- epilogue
-            ok = wait(B::O + w, step - 1);
-            ok = __all_sync(FULL, ok);
-            if (!ok) break;
+            await(B::O + w, step - 1);
             tc_fence_after();
-            const bool live = r < rows;
-            const bool odd0 = odd_flag[(unit & 1) * 2] == unit + 1;
-            const bool odd1 = jd1 > jd0 && odd_flag[(unit & 1) * 2 + 1] == unit + 1;
+            const bool odd = odd_flag[unit & 1] == unit + 1;
             const float inv = l == 0.f ? 0.f : 1.f / l;  // every score -inf: zeros
-            const int64_t row = u.row0 + u.q_lo[w] + (live ? r : 0);
-            const int64_t orow = row * a.out_stride + static_cast<int64_t>(u.head[w]) * a.head_dim;
+            const int64_t orow = (live ? row : 0) * a.out_stride +
+                                 static_cast<int64_t>(head) * a.head_dim;
 #pragma unroll 1
             for (int c = 0; c < DP / 32; ++c) {
                 if (c * 32 >= a.head_dim) break;
                 float o[32];
                 tmem_ld32(to + c * 32, o);
+                if (!live) continue;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] *= inv;
-                if (odd0 || odd1) {
-                    // the entries scrub() took out, for the rows that see them
-                    const __half* vg = static_cast<const __half*>(a.v) + u.row0 * a.kv_stride +
+                if (odd) {  // the entries scrub() took out, for the rows that see them
+                    const __half* vg = static_cast<const __half*>(a.v) +
                                        static_cast<int64_t>(u.kvh) * a.head_dim + c * 32;
-                    for (int ev = 0; ev < 2; ++ev) {
-                        if (!(ev ? odd1 : odd0)) continue;
-                        const int k0 = (ev ? jd1 : jd0) * kTile;
-                        for (int key = k0; key < k0 + kTile && key < u.n && key <= qpos; ++key) {
+                    for (int key = first; key <= row; ++key) {
+                        if (!u.ragged(key / kTile)) {
+                            key |= kTile - 1;  // to the tile's end
+                            continue;
+                        }
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                if (c * 32 + i >= a.head_dim) continue;
-                                const __half hv = vg[key * a.kv_stride + i];
-                                if (odd_half(__half_as_ushort(hv))) o[i] += __half2float(hv);
-                            }
+                        for (int i = 0; i < 32; ++i) {
+                            if (c * 32 + i >= a.head_dim) continue;
+                            const __half hv = vg[key * a.kv_stride + i];
+                            if (odd_half(__half_as_ushort(hv))) o[i] += __half2float(hv);
                         }
                     }
                 }
-                if (!live) continue;
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
                     if (c * 32 + i >= a.head_dim) break;
@@ -582,137 +679,159 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
             }
+            __syncwarp();
             tc_fence_before();
             mbar_arrive(bar(B::E + w));
             if (a.lse && live)
-                a.lse[row * a.q_heads + u.head[w]] =
+                a.lse[static_cast<int64_t>(row) * a.q_heads + head] =
                     ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-        if (warp == 8) {
-            if (lane == 0) {
-                const int nb = (a.head_dim + 63) / 64;  // 64-column boxes that hold anything
-                int ring = 0, cnt[2] = {0, 0};
-                bool ok = true;
-                auto load_q = [&](int i) {
-                    const int qb = cnt[i] % Cfg::QBUF, round = cnt[i] / Cfg::QBUF;
-                    ++cnt[i];
-                    const int b = qb * 2 + i;
-                    if (round > 0) ok = wait(B::QE + b, round - 1);
-                    if (!ok) return;
-                    mbar_arrive_tx(bar(B::QF + b), static_cast<uint32_t>(nb * Cfg::BLK));
-                    for (int c = 0; c < nb; ++c)
-                        tma_load_3d(sbase + b * Cfg::TILE + c * Cfg::BLK, &qmap, c * 64, u.head[i],
-                                    static_cast<int>(u.row0) + u.q_lo[i], bar(B::QF + b));
-                };
-                auto load_kv = [&](const CUtensorMap* map, int j) {
-                    const int st = ring % Cfg::STAGES, round = ring / Cfg::STAGES;
-                    if (round > 0) ok = wait(B::KE + st, round - 1);
-                    if (!ok) return;
-                    ++ring;
-                    mbar_arrive_tx(bar(B::KF + st), static_cast<uint32_t>(nb * Cfg::BLK));
-                    for (int c = 0; c < nb; ++c)
-                        tma_load_3d(sbase + Cfg::OFF_KV + st * Cfg::TILE + c * Cfg::BLK, map, c * 64,
-                                    u.kvh, static_cast<int>(u.row0) + j * kTile, bar(B::KF + st));
-                };
-                while (ok && sched.next(a, u)) {
-                    const int nt = u.nt[1] > u.nt[0] ? u.nt[1] : u.nt[0];
-                    load_q(0);
-                    if (ok) load_kv(&kmap, 0);
-                    if (ok && u.nt[1]) load_q(1);
-                    if (ok) load_kv(&vmap, 0);
-                    for (int j = 1; ok && j < nt; ++j) {
-                        load_kv(&kmap, j);
-                        if (ok) load_kv(&vmap, j);
-                    }
-                }
-                if (!ok) {  // another role gave up: let the copies in flight land
-                    for (int i = ring < Cfg::STAGES ? 0 : ring - Cfg::STAGES; i < ring; ++i)
-                        mbar_drain(bar(B::KF + i % Cfg::STAGES), (i / Cfg::STAGES) & 1);
+        if (warp == 8 && lane == 0) {
+            constexpr int NB = DP / 64;
+            int ring = 0, cnt[2] = {0, 0};
+            bool ok = true;
+            auto load_q = [&](int i) {
+                const int qb = cnt[i] % Cfg::QBUF, round = cnt[i] / Cfg::QBUF;
+                const int b = qb * 2 + i;
+                if (round > 0) ok = wait(B::QE + b, round - 1);
+                if (!ok) return;
+                ++cnt[i];
+                mbar_arrive_tx(bar(B::QF + b), static_cast<uint32_t>(Cfg::TILE));
+                for (int c = 0; c < NB; ++c)
+                    tma_load_3d(sbase + b * Cfg::TILE + c * Cfg::BLK, &qmap, c * 64, u.head[i],
+                                u.tile[i] * kTile, bar(B::QF + b));
+            };
+            auto load_kv = [&](const CUtensorMap* map, int j) {
+                const int st = ring % Cfg::STAGES, round = ring / Cfg::STAGES;
+                if (round > 0) ok = wait(B::KE + st, round - 1);
+                if (!ok) return;
+                ++ring;
+                mbar_arrive_tx(bar(B::KF + st), static_cast<uint32_t>(Cfg::TILE));
+                for (int c = 0; c < NB; ++c)
+                    tma_load_3d(sbase + Cfg::OFF_KV + st * Cfg::TILE + c * Cfg::BLK, map, c * 64,
+                                u.kvh, j * kTile, bar(B::KF + st));
+            };
+            while (ok && sched.template next<Cfg::KS>(a, u)) {
+                for (int j = u.jlo; ok && j <= u.jhi; ++j) {
+                    if (u.on(0) && j == u.lo[0] / SPT) load_q(0);
+                    if (ok) load_kv(&kmap, j);
+                    if (ok && u.on(1) && j == u.lo[1] / SPT) load_q(1);
+                    if (ok) load_kv(&vmap, j);
                 }
             }
-        } else if (warp == 9) {
-            if (lane == 0) {
-                constexpr uint32_t IDESC_QK = f16_idesc(128, 128, false);
-                constexpr uint32_t IDESC_PV = f16_idesc(128, DP, true);
-                const int ksteps = (a.head_dim + 15) / 16;
-                int ring0 = 0, qcnt[2] = {0, 0}, steps[2] = {0, 0}, events[2] = {0, 0};
-                bool ok = true;
-                auto stage_of = [&](int r) { return r % Cfg::STAGES; };
-                auto full = [&](int r) { return wait(B::KF + stage_of(r), r / Cfg::STAGES); };
-                // S_i = Q_i K_j^T.  P_i of the step before lies in S_i's columns: its product has to
-                // be done.
-                auto qk = [&](int i, int j) {
-                    const int r = ring0 + 2 * j, qb = qcnt[i] % Cfg::QBUF;
-                    if (j == 0) ok = wait(B::QF + qb * 2 + i, qcnt[i] / Cfg::QBUF);
-                    ok = ok && full(r);
-                    if (ok && steps[i] > 0) ok = wait(B::O + i, steps[i] - 1);
-                    if (!ok) return;
+            if (!ok) {  // another role gave up: let the copies in flight land
+                for (int i = ring < Cfg::STAGES ? 0 : ring - Cfg::STAGES; i < ring; ++i)
+                    mbar_drain(bar(B::KF + i % Cfg::STAGES), (i / Cfg::STAGES) & 1);
+                for (int i = 0; i < 2; ++i)
+                    for (int n = cnt[i] < Cfg::QBUF ? 0 : cnt[i] - Cfg::QBUF; n < cnt[i]; ++n)
+                        mbar_drain(bar(B::QF + (n % Cfg::QBUF) * 2 + i), (n / Cfg::QBUF) & 1);
+            }
+        } else if (warp == 9 || warp == 10) {
+            // One MMA warp an item: while one waits for its softmax group the other one's
+            // products run.  The whole warp walks this code and one elected lane issues: with
+            // uniform control flow the descriptors stay in uniform registers (issued from a
+            // divergent lane, an MMA took about 100 cycles, against 32 to 64 to execute).
+            constexpr uint32_t IDESC_QK = f16_idesc(128, KS, false);
+            constexpr uint32_t IDESC_PV = f16_idesc(128, DP, true);
+            const int i = warp - 9;
+            const bool leader = elect_one();
+            const int ksteps = (a.head_dim + 15) / 16;
+            const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
+            int ring0 = 0, units = 0, scores = 0, prods = 0, events = 0;
+            auto await = [&](int b, int phase) {
+                mbar_wait_uniform(bar(b), phase & 1, abort_addr, &g_attention_status);
+            };
+            auto stage_of = [&](int x) { return x % Cfg::STAGES; };
+            auto await_full = [&](int x) { await(B::KF + stage_of(x), x / Cfg::STAGES); };
+            int lo = 0, hi = 0;  // this item's steps
+            // S = Q K^T of step n, if the item has it, over scores that were read.  Every K tile is
+            // given back once, by both warps.
+            auto qk = [&](int n) {
+                const int sub = n % SPT;
+                const int x = ring0 + 2 * (n / SPT - u.jlo), qb = units % Cfg::QBUF;
+                const bool mine = n >= lo && n <= hi;
+                if (sub == 0) await_full(x);  // each tile, to stay in step with the other warp
+                if (mine) {
+                    if (n == lo) await(B::QF + qb * 2 + i, units / Cfg::QBUF);
+                    if (scores > 0) await(B::F + i, scores - 1);
                     tc_fence_after();
-                    const uint32_t qa = sbase + (qb * 2 + i) * Cfg::TILE;
-                    const uint32_t ka = sbase + Cfg::OFF_KV + stage_of(r) * Cfg::TILE;
-                    for (int kk = 0; kk < ksteps; ++kk) {
-                        const uint32_t off = (kk >> 2) * Cfg::BLK + (kk & 3) * 32;
-                        tc_mma(tmem_s(i), sw128_desc(qa + off, 16, 1024),
-                               sw128_desc(ka + off, 16, 1024), IDESC_QK, kk > 0);
-                    }
-                    tc_commit(bar(B::S + i));
-                    if (i == 1 || u.nt[1] == 0) tc_commit(bar(B::KE + stage_of(r)));
-                    if (j == u.nt[i] - 1) {
-                        tc_commit(bar(B::QE + qb * 2 + i));
-                    }
-                };
-                auto pv = [&](int i, int j) {
-                    const int r = ring0 + 2 * j + 1;
-                    ok = wait(B::P + i, steps[i]) && full(r);
-                    // the accumulator still holds this item's previous unit
-                    if (ok && j == 0 && qcnt[i] > 0) ok = wait(B::E + i, qcnt[i] - 1);
-                    if (!ok) return;
-                    tc_fence_after();
-                    const uint32_t va = sbase + Cfg::OFF_KV + stage_of(r) * Cfg::TILE;
-    #pragma unroll
-                    for (int kk = 0; kk < kTile / 16; ++kk)
-                        tc_mma_ts(tmem_o(i), tmem_s(i) + 8u * kk,
-                                  sw128_desc(va + kk * 2048, Cfg::BLK, 1024), IDESC_PV,
-                                  j > 0 || kk > 0);
-                    tc_commit(bar(B::O + i));
-                    ++steps[i];
-                    if (i == 1 || u.nt[1] == 0) tc_commit(bar(B::KE + stage_of(r)));
-                };
-                // the diagonal tile's V has landed: the softmax groups may scrub it
-                auto v_ready = [&](int j, int event) {
-                    ok = ok && full(ring0 + 2 * j + 1);
-                    if (ok) mbar_arrive(bar(B::VR + event));
-                };
-                while (ok && sched.next(a, u)) {
-                    const int nt = u.nt[1] > u.nt[0] ? u.nt[1] : u.nt[0];
-                    const int jd0 = u.nt[0] - 1, jd1 = u.nt[1] - 1;
-                    qk(0, 0);
-                    if (ok && u.nt[1]) qk(1, 0);
-                    if (jd0 == 0) v_ready(0, 0);
-                    for (int j = 0; ok && j < nt; ++j) {
-                        // a diagonal tile's V is scrubbed by both softmax groups first
-                        if (ok && (j == jd0 || j == jd1)) {
-                            const int ev = j == jd0 ? 0 : 1;
-                            ok = wait(B::SB + ev, events[ev]++);
-                        }
-                        if (ok && j < u.nt[0]) {
-                            pv(0, j);
-                            if (ok && j + 1 < u.nt[0]) qk(0, j + 1);
-                            if (j + 1 == jd0) v_ready(j + 1, 0);
-                        }
-                        if (ok && j < u.nt[1]) {
-                            pv(1, j);
-                            if (ok && j + 1 < u.nt[1]) qk(1, j + 1);
-                            if (j + 1 == jd1 && jd1 > jd0) v_ready(j + 1, 1);
-                        }
-                    }
-                    ring0 += 2 * nt;
-                    ++qcnt[0];
-                    if (u.nt[1]) ++qcnt[1];
                 }
-                tc_commit(bar(B::DONE));  // every product is done before the CTA frees its memory
+                const uint32_t qa = sbase + (qb * 2 + i) * Cfg::TILE;
+                const uint32_t ka = sbase + Cfg::OFF_KV + stage_of(x) * Cfg::TILE + sub * KS * 128;
+                const uint64_t qd = sw128_desc(qa, 16, 1024), kd = sw128_desc(ka, 16, 1024);
+                const uint32_t d = tmem_s(i);
+                if (leader) {
+                    if (mine) {
+#pragma unroll
+                        for (int kk = 0; kk < DP / 16; ++kk) {
+                            const uint32_t off = ((kk >> 2) * Cfg::BLK + (kk & 3) * 32) >> 4;
+                            if (kk < ksteps) tc_mma(d, qd + off, kd + off, IDESC_QK, kk > 0);
+                        }
+                        tc_commit(bar(B::S + i));
+                        if (n == hi) tc_commit(bar(B::QE + qb * 2 + i));
+                    }
+                    if (sub == SPT - 1) tc_commit(bar(B::KE + stage_of(x)));
+                }
+                __syncwarp();
+                if (mine) ++scores;
+            };
+            auto pv = [&](int n) {
+                const int sub = n % SPT;
+                const int x = ring0 + 2 * (n / SPT - u.jlo) + 1;
+                const bool mine = n >= lo && n <= hi;
+                if (sub == 0) await_full(x);
+                if (mine) {
+                    await(B::P + i, prods);
+                    // the accumulator still holds this item's previous unit
+                    if (n == lo && units > 0) await(B::E + i, units - 1);
+                    tc_fence_after();
+                }
+                const uint32_t va = sbase + Cfg::OFF_KV + stage_of(x) * Cfg::TILE + sub * KS * 128;
+                const uint64_t vd = sw128_desc(va, Cfg::BLK, 1024);
+                const uint32_t d = tmem_o(i), p = tmem_p(i);
+                if (leader) {
+                    if (mine) {
+#pragma unroll
+                        for (int kk = 0; kk < KS / 16; ++kk)
+                            tc_mma_ts(d, p + 8u * kk, vd + kk * (2048 >> 4), IDESC_PV,
+                                      n > lo || kk > 0);
+                        tc_commit(bar(B::O + i));
+                    }
+                    if (sub == SPT - 1) tc_commit(bar(B::KE + stage_of(x)));
+                }
+                __syncwarp();
+                if (mine) ++prods;
+            };
+            // a V tile to scrub has landed
+            auto v_ready = [&](int n) {
+                if (n % SPT || !u.ragged(n / SPT)) return;
+                await_full(ring0 + 2 * (n / SPT - u.jlo) + 1);
+                if (leader) mbar_arrive(bar(B::VR));
+                __syncwarp();
+            };
+            while (sched.template next<Cfg::KS>(a, u) && !*abort_flag) {
+                u.make_uniform();
+                lo = i ? u.lo[1] : u.lo[0];
+                hi = i ? u.hi[1] : u.hi[0];
+                const int n0 = u.jlo * SPT, n1 = u.jhi * SPT + SPT - 1;
+                qk(n0);
+                v_ready(n0);
+                for (int n = n0; n <= n1; ++n) {
+                    if (n % SPT == 0 && u.ragged(n / SPT)) await(B::SB, events++);
+                    if (n < n1) {
+                        qk(n + 1);
+                        v_ready(n + 1);
+                    }
+                    pv(n);
+                }
+                ring0 += 2 * (u.jhi - u.jlo + 1);
+                if (lo <= hi) ++units;
+            }
+            __syncwarp();
+            if (leader) {  // every product is done before the CTA frees its memory
+                tc_commit(bar(B::DONE));
                 mbar_drain(bar(B::DONE), 0);
             }
         }
@@ -746,18 +865,16 @@ int launch_tc(PromptArgs a, cudaStream_t s) {
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
     const int sms = device_sm_count();
-    const int total = a.num_seqs;
-    const int32_t* starts = a.q_start;
-    for (int s0 = 0; s0 < total; s0 += kMaxSeqs) {  // a launch schedules up to 1024 sequences
-        a.num_seqs = total - s0 < kMaxSeqs ? total - s0 : kMaxSeqs;
-        a.q_start = starts + s0;
-        // at most one ragged tile a sequence
-        const int64_t items = ((a.rows + kTile - 1) / kTile + a.num_seqs) * a.q_heads;
+    const int64_t tiles = (a.rows + kTile - 1) / kTile;
+    for (int64_t t0 = 0; t0 < tiles; t0 += kWindow) {
+        const int64_t n = tiles - t0 < kWindow ? tiles - t0 : kWindow;
+        const int64_t items = n * a.q_heads;
         if (items > INT32_MAX) return fail(TMLLM_INVALID_SHAPE, "too many prompt tiles");
-        a.pairs = items > 2 * sms;
+        // one item a unit while that still leaves SMs idle
+        a.pairs = items <= sms ? 0 : a.group % 2 == 0 ? 1 : 2;
         const int64_t ctas = items < sms ? items : sms;
-        prompt_tc_kernel<DP><<<static_cast<unsigned>(ctas), kTcThreads, Cfg::SMEM, s>>>(qmap, kmap,
-                                                                                       vmap, a);
+        prompt_tc_kernel<DP><<<static_cast<unsigned>(ctas), kTcThreads, Cfg::SMEM, s>>>(
+            qmap, kmap, vmap, a, static_cast<int>(t0));
         TMLLM_LAUNCH_TRY();
     }
     return TMLLM_OK;
@@ -860,8 +977,7 @@ int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, c
     if (dtype == TMLLM_F32) return launch_fma_d<float>(a, s);
     const bool tc = head_dim % 8 == 0 && head_dim <= 128 && q_stride % 8 == 0 &&
                     kv_stride % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) &&
-                    aligned16(out) && max_rows <= kMaxLevels * kTile &&
-                    q_stride < (int64_t{1} << 38) && kv_stride < (int64_t{1} << 38);
+                    aligned16(out) && q_stride < (int64_t{1} << 38) && kv_stride < (int64_t{1} << 38);
     if (!tc) return launch_fma_d<__half>(a, s);
     return head_dim <= 64 ? launch_tc<64>(a, s) : launch_tc<128>(a, s);
 }
