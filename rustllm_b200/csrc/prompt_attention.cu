@@ -220,7 +220,7 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 // sequence starts, all tiles of an item whose rows belong to several sequences).
 constexpr int kTile = 128;
 constexpr int kTcThreads = 384;  // warp 11 completes a warpgroup and idles
-constexpr int kWindow = 2048;    // row tiles a launch schedules (262,144 packed rows)
+constexpr int kWindow = 1024;    // row tiles a launch schedules (131,072 packed rows)
 
 template <int DP>
 struct AttCfg {
@@ -231,8 +231,10 @@ struct AttCfg {
     static constexpr int OFF_KV = 2 * QBUF * TILE;
     static constexpr int OFF_SEQ = OFF_KV + STAGES * TILE;      // int32 sequence of a tile's first row
     static constexpr int OFF_HIST = OFF_SEQ + kWindow * 4;      // int32 row tiles of each cost
-    static constexpr int OFF_LIST = OFF_HIST + kWindow * 4;     // uint16 row tiles, longest first
-    static constexpr int OFF_BAR = OFF_LIST + kWindow * 2;
+    static constexpr int OFF_COST = OFF_HIST + kWindow * 4;     // uint16 key tiles of an entry
+    static constexpr int OFF_LIST = OFF_COST + kWindow * 2;     // uint16 entries, longest first
+    static constexpr int OFF_OUT = OFF_LIST + kWindow * 2;      // a warp's 32 rows x 64 bytes, x 8
+    static constexpr int OFF_BAR = OFF_OUT + 8 * 2048;
     static constexpr int KS = DP == 64 ? 128 : 64;  // keys of a step
     static constexpr int SPT = 128 / KS;            // steps of a key tile
     static_assert(3 * KS + 2 * DP <= 512, "tensor memory");
@@ -241,17 +243,16 @@ struct AttCfg {
 };
 
 // Barriers: QF/QE Q tile full / empty, KF/KE ring full / empty; of each item: S scores ready, F
-// scores read, P probabilities written, O product done, E accumulator read; VR a V tile to scrub
-// has landed, SB it is scrubbed, DONE all products.  Both softmax groups and both MMA warps take
-// part in every scrub (every unit has one, its diagonal) and both MMA warps give back every K and
-// V tile, whether their item uses it or not, so no thread ever falls more than a phase behind a
-// barrier that it waits on.
+// scores read, P probabilities written, O product done, E accumulator read, VR a V tile to scrub
+// has landed, SB it is scrubbed; DONE all products.  Both MMA warps give back every K and V tile,
+// whether their item uses it or not, so neither falls more than a phase behind the ring, and a
+// softmax group follows its MMA warp step by step.
 template <int DP>
 struct AttBar {
     using Cfg = AttCfg<DP>;
     static constexpr int QF = 0, QE = QF + 2 * Cfg::QBUF, KF = QE + 2 * Cfg::QBUF,
                          KE = KF + Cfg::STAGES, S = KE + Cfg::STAGES, F = S + 2, P = F + 2,
-                         O = P + 2, E = O + 2, VR = E + 2, SB = VR + 1, DONE = SB + 1,
+                         O = P + 2, E = O + 2, VR = E + 2, SB = VR + 2, DONE = SB + 2,
                          COUNT = DONE + 1;
     static_assert(COUNT * 8 + 64 <= 512, "barrier area");
 };
@@ -381,17 +382,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     auto bar = [&](int i) { return bars + 8u * static_cast<uint32_t>(i); };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + B::COUNT * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* odd_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [unit parity]
+    volatile int* odd_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);  // scrub found any
     constexpr unsigned FULL = 0xffffffffu;
 
     if (tid == 0) {
         for (int i = 0; i < B::COUNT; ++i) {
-            const bool group = i >= B::F && i < B::E + 2 && !(i >= B::O && i < B::O + 2);
-            const bool both = i == B::VR || i == B::DONE || (i >= B::KE && i < B::KE + Cfg::STAGES);
-            mbar_init(bar(i), i == B::SB ? 256u : group ? 128u : both ? 2u : 1u);
+            const bool group = (i >= B::F && i < B::O) || (i >= B::E && i < B::VR) ||
+                               (i >= B::SB && i < B::DONE);
+            const bool both = i == B::DONE || (i >= B::KE && i < B::KE + Cfg::STAGES);
+            mbar_init(bar(i), group ? 128u : both ? 2u : 1u);
         }
         *abort_flag = 0;
-        odd_flag[0] = odd_flag[1] = 0;
+        *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) {
@@ -405,6 +407,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int32_t* tile_seq = reinterpret_cast<int32_t*>(smem + Cfg::OFF_SEQ);
     int32_t* hist = reinterpret_cast<int32_t*>(smem + Cfg::OFF_HIST);
     uint16_t* list = reinterpret_cast<uint16_t*>(smem + Cfg::OFF_LIST);
+    uint16_t* cost = reinterpret_cast<uint16_t*>(smem + Cfg::OFF_COST);
     AttSched sched{tile_seq, list, 0, 0, tile0, 0, 0, 0};
     {
         const int q0 = __ldg(a.q_start), q1 = __ldg(a.q_start + a.num_seqs);
@@ -421,11 +424,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         sched.total = count * sched.per;
         const bool sorted = sched.total > static_cast<int>(gridDim.x);
         for (int i = tid; i < kWindow; i += kTcThreads) hist[i] = 0;
-        auto cost_of = [&](int e) {
-            const int t0 = max(e * span, ta), t1 = min(e * span + span, tb) - 1;
-            const int c = tile0 + t1 - max(__ldg(a.q_start + tile_seq[t0]), 0) / kTile;
-            return c < kWindow ? c : kWindow - 1;
-        };
         for (int t = ta + tid; t < tb; t += kTcThreads) {
             const int row = (tile0 + t) * kTile;
             tile_seq[t] = seq_at(a, row > sched.row_lo ? row : sched.row_lo, 0);
@@ -434,7 +432,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!sorted) {
             for (int i = tid; i < count; i += kTcThreads) list[i] = static_cast<uint16_t>(ea + i);
         } else {
-            for (int i = tid; i < count; i += kTcThreads) atomicAdd(hist + cost_of(ea + i), 1);
+            for (int i = tid; i < count; i += kTcThreads) {
+                const int t0 = max((ea + i) * span, ta), t1 = min((ea + i) * span + span, tb) - 1;
+                const int c = tile0 + t1 - max(__ldg(a.q_start + tile_seq[t0]), 0) / kTile;
+                cost[i] = static_cast<uint16_t>(c < kWindow ? c : kWindow - 1);
+                atomicAdd(hist + cost[i], 1);
+            }
             __syncthreads();
             if (warp == 0) {
                 int above = 0;  // entries of a higher cost
@@ -454,7 +457,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // in order within a cost, so every CTA has the same list
                 for (int i0 = 0; i0 < count; i0 += 32) {
                     const int i = i0 + lane;
-                    const int c = i < count ? cost_of(ea + i) : -1;
+                    const int c = i < count ? cost[i] : -1;
                     const unsigned same = __match_any_sync(FULL, c);
                     const int before = __popc(same & ((1u << lane) - 1u));
                     const int at = c >= 0 ? hist[c] : 0;
@@ -489,40 +492,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem_s(w) + lane_base, to = tmem_o(w) + lane_base;
         const uint32_t tp = tmem_p(w) + lane_base;
+        unsigned char* stage = smem + Cfg::OFF_OUT + warp * 2048;
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
-        int step = 0, ring0 = 0, unit = 0, events = 0;
+        int step = 0, ring0 = 0, events = 0;
         auto await = [&](int b, int phase) {
             mbar_wait_uniform(bar(b), phase & 1, abort_addr, &g_attention_status);
         };
-        // Non-finite entries of the V tile of key tile j become zeros (and raise the unit's
-        // flag); all 256 softmax threads share the tile.
+        // Non-finite entries of the V tile of key tile j become zeros, and the flag says that some
+        // were found.  Each group does it for its own item: the other one may be on the same
+        // tile, writing the same zeros (the flag comes first, so who sees a zero sees the flag).
         auto scrub = [&](int j) {
             const int st = (ring0 + 2 * (j - u.jlo) + 1) % Cfg::STAGES;
-            await(B::VR, events++);
-            unsigned char* v = smem + Cfg::OFF_KV + st * Cfg::TILE + tid * 16;
+            await(B::VR + w, events++);
+            unsigned char* v = smem + Cfg::OFF_KV + st * Cfg::TILE + r * 16;
             __half2 probe = __floats2half2_rn(0.f, 0.f);
             const __half2 zero = probe;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) {
-                const uint4 x = *reinterpret_cast<const uint4*>(v + 4096 * c);
+            for (int c = 0; c < DP / 8; ++c) {
+                const uint4 x = *reinterpret_cast<const uint4*>(v + 2048 * c);
                 const __half2* h = reinterpret_cast<const __half2*>(&x);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) probe = __hfma2(h[e], zero, probe);  // 0 or NaN
             }
             if (!(__low2float(probe) == 0.f && __high2float(probe) == 0.f)) {
-                odd_flag[unit & 1] = unit + 1;
-                for (int c = 0; c < DP / 16; ++c) {
-                    __half* p = reinterpret_cast<__half*>(v + 4096 * c);
-                    for (int e = 0; e < 8; ++e)
-                        if (odd_half(__half_as_ushort(p[e]))) p[e] = __float2half_rn(0.f);
+                *odd_flag = 1;
+                __threadfence_block();
+                for (int c = 0; c < DP / 8; ++c) {
+                    for (int e = 0; e < 8; ++e) {
+                        volatile uint16_t* b = reinterpret_cast<volatile uint16_t*>(v + 2048 * c) + e;
+                        if (odd_half(*b)) *b = 0;
+                    }
                 }
             }
+            __threadfence_block();
             __syncwarp();
             fence_async_smem();
-            mbar_arrive(bar(B::SB));
+            mbar_arrive(bar(B::SB + w));
         };
         const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-        for (; sched.template next<Cfg::KS>(a, u) && !*abort_flag; ++unit) {
+        while (sched.template next<Cfg::KS>(a, u) && !*abort_flag) {
             const int lo = w ? u.lo[1] : u.lo[0], hi = w ? u.hi[1] : u.hi[0];
             const int tile = w ? u.tile[1] : u.tile[0], head = w ? u.head[1] : u.head[0];
             const int row = tile * kTile + r;  // keys `first` .. row are visible
@@ -535,26 +543,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 first = max(__ldg(a.q_start + (several ? seq_at(a, row, s0) : s0)), 0);
             }
             float m = -INFINITY, l = 0.f;
-            for (int n = u.jlo * SPT; n <= u.jhi * SPT + SPT - 1; ++n) {
+            for (int n = lo; n <= hi; ++n) {
                 const bool ragged = u.ragged(n / SPT);
-                if (ragged && n % SPT == 0) scrub(n / SPT);
-                if (n < lo || n > hi) continue;
+                if (ragged && (n % SPT == 0 || n == lo)) scrub(n / SPT);
                 await(B::S + w, step);
                 tc_fence_after();
                 float v[KS];
                 tmem_ld_row(ts, v);
                 tc_fence_before();
                 mbar_arrive(bar(B::F + w));
-                int dark_lo = 0, dark_hi = KS - 1;  // columns some row of the warp sees
+                // of each 32 columns: every row of the warp sees all of them (mask without
+                // work), none sees any (no exponentials either), or something between
+                uint32_t dark = 0;  // bit c: 32 columns from 32 c on are dark
                 if (ragged) {
                     // columns c_lo .. c_hi of this row are visible
                     const int c_lo = live ? first - n * KS : KS;
                     const int c_hi = live ? row - n * KS : -1;
-                    dark_lo = __reduce_min_sync(FULL, c_lo);
-                    dark_hi = __reduce_max_sync(FULL, c_hi);
+                    const int some_lo = __reduce_min_sync(FULL, c_lo);
+                    const int some_hi = __reduce_max_sync(FULL, c_hi);
+                    const int all_lo = __reduce_max_sync(FULL, c_lo);
+                    const int all_hi = __reduce_min_sync(FULL, c_hi);
 #pragma unroll
-                    for (int i = 0; i < KS; ++i)
-                        v[i] = (i >= c_lo && i <= c_hi) ? v[i] : -INFINITY;
+                    for (int c = 0; c < KS / 32; ++c) {
+                        if (c * 32 > some_hi || c * 32 + 31 < some_lo) dark |= 1u << c;
+                        if (c * 32 < all_lo || c * 32 + 31 > all_hi) {
+                            auto below = [](int x) {  // bits 0 .. x - 1
+                                return x <= 0 ? 0u : x >= 32 ? ~0u : (1u << x) - 1u;
+                            };
+                            const uint32_t see = below(c_hi + 1 - c * 32) & ~below(c_lo - c * 32);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                v[c * 32 + i] = (see & (1u << i)) ? v[c * 32 + i] : -INFINITY;
+                        }
+                    }
                 }
                 auto row_max = [&]() {
                     float mx[4] = {v[0], v[1], v[2], v[3]};
@@ -570,15 +591,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // known at once, and this step's own maximum is found meanwhile.  Only when it
                 // exceeds m by more than 2^8 does m follow (P is computed again, O and l are
                 // rescaled); else P stays below 2^8 and 1 / l makes up for it.
+                // A row's first visible step (m = -inf: its l and O are zero) takes its maximum.
                 const bool begin = n == lo;
-                if (begin) m = row_max();
+                const bool fresh = m == -INFINITY;
+                if (__any_sync(FULL, fresh)) {
+                    const float mt = row_max();
+                    if (fresh) m = mt;
+                }
                 float alpha = 1.f;
                 bool grown = false;  // of some row of the warp
                 float2 l2[2];
-                if (!begin) {  // the product before has read P
-                    await(B::O + w, step - 1);
-                    tc_fence_after();
-                }
                 for (;;) {
                     // -inf (nothing visible yet): exp2(-inf - 0) = 0
                     const float sub = m == -INFINITY ? 0.f : -m;
@@ -588,7 +610,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int c = 0; c < KS / 32; ++c) {
                         uint32_t pk[16];
                         // 32 columns no row of the warp sees: zeros without exponentials
-                        if (c * 32 <= dark_hi && c * 32 + 31 >= dark_lo) {
+                        if (!(dark >> c & 1u)) {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 const int i = c * 32 + 2 * e;
@@ -601,15 +623,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                             for (int e = 0; e < 16; ++e) pk[e] = 0u;
                         }
+                        if (c == 0 && !begin) {  // the product before has read P
+                            await(B::O + w, step - 1);
+                            tc_fence_after();
+                        }
                         tmem_st16_bits(tp + 16 * c, pk);
                     }
-                    if (begin) break;
+                    if (begin || dark == (1u << (KS / 32)) - 1u) break;
                     const float mt = row_max();
                     const bool grow = mt > m + 8.f;
                     if (!__any_sync(FULL, grow)) break;
                     grown = true;
                     if (grow) {
-                        alpha = m == -INFINITY ? 0.f : exp2_approx(m - mt);
+                        alpha = exp2_approx(m - mt);
                         l *= alpha;
                         m = mt;
                     }
@@ -635,7 +661,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ---- epilogue
             await(B::O + w, step - 1);
             tc_fence_after();
-            const bool odd = odd_flag[unit & 1] == unit + 1;
+            const bool odd = *odd_flag != 0;
             const float inv = l == 0.f ? 0.f : 1.f / l;  // every score -inf: zeros
             const int64_t orow = (live ? row : 0) * a.out_stride +
                                  static_cast<int64_t>(head) * a.head_dim;
@@ -644,10 +670,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (c * 32 >= a.head_dim) break;
                 float o[32];
                 tmem_ld32(to + c * 32, o);
-                if (!live) continue;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] *= inv;
-                if (odd) {  // the entries scrub() took out, for the rows that see them
+                if (odd && live) {  // the entries scrub() took out, for the rows that see them
                     const __half* vg = static_cast<const __half*>(a.v) +
                                        static_cast<int64_t>(u.kvh) * a.head_dim + c * 32;
                     for (int key = first; key <= row; ++key) {
@@ -663,21 +688,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                     }
                 }
+                if (a.out_f32) {
+                    if (!live) continue;
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (c * 32 + i >= a.head_dim) break;
-                    if (a.out_f32) {
+                    for (int i = 0; i < 32; i += 8) {
+                        if (c * 32 + i >= a.head_dim) break;
                         float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.out) + orow +
                                                                 c * 32 + i);
                         dst[0] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                         dst[1] = make_float4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]);
-                    } else {
-                        *reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + orow + c * 32 + i) =
-                            make_uint4(pack_half2(o[i], o[i + 1]), pack_half2(o[i + 2], o[i + 3]),
-                                       pack_half2(o[i + 4], o[i + 5]),
-                                       pack_half2(o[i + 6], o[i + 7]));
                     }
+                    continue;
                 }
+                // through shared memory, so that four lanes write a row's 64 bytes together
+                // (straight from the registers every store would touch 32 rows)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)) =
+                        make_uint4(pack_half2(o[8 * i], o[8 * i + 1]),
+                                   pack_half2(o[8 * i + 2], o[8 * i + 3]),
+                                   pack_half2(o[8 * i + 4], o[8 * i + 5]),
+                                   pack_half2(o[8 * i + 6], o[8 * i + 7]));
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int sr = i * 8 + (lane >> 2), sc = lane & 3;  // row and 16-byte chunk
+                    const int srow = row - lane + sr;
+                    const uint4 x = *reinterpret_cast<const uint4*>(
+                        stage + sr * 64 + ((sc ^ (sr >> 1 & 3)) << 4));
+                    if (srow >= sched.row_lo && srow < sched.row_hi &&
+                        c * 32 + sc * 8 < a.head_dim)
+                        *reinterpret_cast<uint4*>(static_cast<__half*>(a.out) +
+                                                  srow * a.out_stride +
+                                                  static_cast<int64_t>(head) * a.head_dim + c * 32 +
+                                                  sc * 8) = x;
+                }
+                __syncwarp();
             }
             __syncwarp();
             tc_fence_before();
@@ -804,11 +850,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 if (mine) ++prods;
             };
-            // a V tile to scrub has landed
+            // step n's is the item's first use of a V tile that is scrubbed before
+            auto scrubs = [&](int n) {
+                return n >= lo && n <= hi && (n % SPT == 0 || n == lo) && u.ragged(n / SPT);
+            };
             auto v_ready = [&](int n) {
-                if (n % SPT || !u.ragged(n / SPT)) return;
+                if (!scrubs(n)) return;
                 await_full(ring0 + 2 * (n / SPT - u.jlo) + 1);
-                if (leader) mbar_arrive(bar(B::VR));
+                if (leader) mbar_arrive(bar(B::VR + i));
                 __syncwarp();
             };
             while (sched.template next<Cfg::KS>(a, u) && !*abort_flag) {
@@ -819,7 +868,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 qk(n0);
                 v_ready(n0);
                 for (int n = n0; n <= n1; ++n) {
-                    if (n % SPT == 0 && u.ragged(n / SPT)) await(B::SB, events++);
+                    if (scrubs(n)) await(B::SB + i, events++);
                     if (n < n1) {
                         qk(n + 1);
                         v_ready(n + 1);
