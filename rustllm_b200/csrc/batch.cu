@@ -281,6 +281,97 @@ __global__ void __launch_bounds__(256) rope_append_scalar_kernel(const AppendArg
     }
 }
 
+// 16-byte form (D / 2 a multiple of a 16-byte chunk, aligned rows).  A warp takes one row (or a
+// share of its heads): lane = (head of the pass, chunk c of the first half), so a lane's chunk -
+// and with it its cos / sin entries - stays the same while it walks the heads, and the tables are
+// read once a row.  kUnroll heads are loaded before the first is used.
+// Bound by memory: every element is read once and written once or twice (cache and dense).
+template <typename T>
+__global__ void __launch_bounds__(256) rope_append_vec_kernel(const AppendArgs a, int parts) {
+    constexpr int EPC = 16 / sizeof(T), kUnroll = 4;
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int64_t row = unit / parts;
+    const int part = static_cast<int>(unit - row * parts);
+    if (row >= a.rows) return;
+    const int half = a.head_dim / 2, cph = half / EPC, hpp = 32 / cph;  // heads a pass
+    const int hl = lane / cph, c = lane - hl * cph;
+    const int pos = __ldg(a.positions + row);
+    if (pos < 0 || hl >= hpp) return;
+    const int64_t slot = __ldg(a.slots + row);
+    const bool cached = slot >= 0 && slot < a.arena_slots;
+    int64_t cell = 0;  // element of (block, head 0, offset) in the arenas
+    if (cached) {
+        const int64_t blk = (slot >> 32) ? slot / a.block_size
+                                         : static_cast<uint32_t>(slot) / a.block_size;
+        cell = (blk * a.kv_heads * a.block_size + (slot - blk * a.block_size)) * a.head_dim;
+    }
+    const int64_t head_step = static_cast<int64_t>(a.block_size) * a.head_dim;
+    float cs[EPC], sn[EPC];
+    const bool turn = a.cos_table != nullptr && pos < a.rope_len;
+    if (turn) {
+        const int64_t e = static_cast<int64_t>(pos) * half + c * EPC;
+#pragma unroll
+        for (int i = 0; i < EPC; i += 4) {
+            const float4 x = __ldg(reinterpret_cast<const float4*>(a.cos_table + e + i));
+            const float4 y = __ldg(reinterpret_cast<const float4*>(a.sin_table + e + i));
+            cs[i] = x.x, cs[i + 1] = x.y, cs[i + 2] = x.z, cs[i + 3] = x.w;
+            sn[i] = y.x, sn[i + 1] = y.y, sn[i + 2] = y.z, sn[i + 3] = y.w;
+        }
+    }
+    const int heads = a.q_heads + 2 * a.kv_heads;
+    const T* qr = static_cast<const T*>(a.q) + row * a.q_stride + c * EPC;
+    const T* kr = static_cast<const T*>(a.k) + row * a.kv_stride + c * EPC;
+    const T* vr = static_cast<const T*>(a.v) + row * a.kv_stride + c * EPC;
+    for (int h0 = part * hpp + hl; h0 < heads; h0 += kUnroll * parts * hpp) {
+        uint4 x1[kUnroll], x2[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const int h = h0 + k * parts * hpp;
+            if (h >= heads) break;
+            const T* src = h < a.q_heads ? qr + static_cast<int64_t>(h) * a.head_dim
+                           : h < a.q_heads + a.kv_heads
+                               ? kr + static_cast<int64_t>(h - a.q_heads) * a.head_dim
+                               : vr + static_cast<int64_t>(h - a.q_heads - a.kv_heads) * a.head_dim;
+            x1[k] = *reinterpret_cast<const uint4*>(src);
+            x2[k] = *reinterpret_cast<const uint4*>(src + half);
+        }
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const int h = h0 + k * parts * hpp;
+            if (h >= heads) break;
+            const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
+            if (turn && !is_v) {
+                float f1[EPC], f2[EPC];
+                Chunk<T>::unpack(x1[k], f1);
+                Chunk<T>::unpack(x2[k], f2);
+                T* p1 = reinterpret_cast<T*>(&x1[k]);
+                T* p2 = reinterpret_cast<T*>(&x2[k]);
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) {
+                    rotate(f1[e], f2[e], cs[e], sn[e]);
+                    p1[e] = from_f32<T>(f1[e]);
+                    p2[e] = from_f32<T>(f2[e]);
+                }
+            }
+            const int kvh = is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
+            if (is_q || (!is_v && a.k_out)) {
+                T* o = is_q ? static_cast<T*>(a.q_out) + row * a.qo_stride +
+                                  static_cast<int64_t>(h) * a.head_dim + c * EPC
+                            : static_cast<T*>(a.k_out) + row * a.ko_stride +
+                                  static_cast<int64_t>(kvh) * a.head_dim + c * EPC;
+                *reinterpret_cast<uint4*>(o) = x1[k];
+                *reinterpret_cast<uint4*>(o + half) = x2[k];
+            }
+            if (!is_q && cached) {
+                T* o = static_cast<T*>(is_v ? a.v_cache : a.k_cache) + cell + kvh * head_step + c * EPC;
+                *reinterpret_cast<uint4*>(o) = x1[k];
+                *reinterpret_cast<uint4*>(o + half) = x2[k];
+            }
+        }
+    }
+}
+
 int grid_of(int64_t items) {
     int64_t blocks = (items + 255) / 256;
     const int64_t cap = static_cast<int64_t>(device_sm_count()) * 32;
@@ -422,10 +513,34 @@ int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, co
     a.head_dim = kv->head_dim;
     a.block_size = kv->block_size;
     a.rope_len = rope_len;
-    const int nb = grid_of(rows * (q_heads + 2 * Hkv) * (D / 2));
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (kv->dtype == TMLLM_F16) rope_append_scalar_kernel<__half><<<nb, 256, 0, s>>>(a);
-    else rope_append_scalar_kernel<float><<<nb, 256, 0, s>>>(a);
+    const int64_t epc = 16 / static_cast<int64_t>(es);
+    bool vec = (D / 2) % epc == 0 && D / 2 / epc <= 32 && q_stride % epc == 0 &&
+               kv_stride % epc == 0 && q_out_stride % epc == 0 && k_out_stride % epc == 0 &&
+               (!rope_cos || (aligned16(rope_cos) && aligned16(rope_sin)));
+    for (const void* p : {q, k, v, static_cast<const void*>(q_out),
+                          static_cast<const void*>(k_out), static_cast<const void*>(kv->k_cache),
+                          static_cast<const void*>(kv->v_cache)})
+        vec = vec && aligned16(p);
+    if (vec) {
+        // a warp a row; few rows: as many warps a row as its heads give, up to 8 warps an SM
+        const int64_t passes = (q_heads + 2 * Hkv) * (D / 2 / epc) / 32 + 1;
+        int64_t parts = static_cast<int64_t>(device_sm_count()) * 8 / rows;
+        if (parts > passes) parts = passes;
+        if (parts < 1) parts = 1;
+        const int64_t ctas = (rows * parts + 7) / 8;
+        if (ctas > INT32_MAX) return fail(TMLLM_INVALID_SHAPE, "too many rows");
+        if (kv->dtype == TMLLM_F16)
+            rope_append_vec_kernel<__half>
+                <<<static_cast<unsigned>(ctas), 256, 0, s>>>(a, static_cast<int>(parts));
+        else
+            rope_append_vec_kernel<float>
+                <<<static_cast<unsigned>(ctas), 256, 0, s>>>(a, static_cast<int>(parts));
+    } else {
+        const int nb = grid_of(rows * (q_heads + 2 * Hkv) * (D / 2));
+        if (kv->dtype == TMLLM_F16) rope_append_scalar_kernel<__half><<<nb, 256, 0, s>>>(a);
+        else rope_append_scalar_kernel<float><<<nb, 256, 0, s>>>(a);
+    }
     TMLLM_LAUNCH_TRY();
     return TMLLM_OK;
 }
