@@ -77,7 +77,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform for the compiler too
     const uint32_t bars = sbase + Cfg::OFF_BAR;
     auto full = [&](int i) { return bars + 8u * i; };
     auto empty = [&](int i) { return bars + 8u * (Cfg::STAGES + i); };
@@ -142,38 +143,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_drain(full(i % Cfg::STAGES), (i / Cfg::STAGES) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t IDESC = f16_idesc(kM, BN, true);
-            int g = 0, it = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x, ++it) {
-                const int ab = it & 1;
-                if (it >= 2) {
-                    ok = mbar_wait_bounded(acc_empty(ab), ((it >> 1) - 1) & 1, abort_flag,
-                                           &g_linear_status);
-                    if (!ok) break;
-                    tc_fence_after();
-                }
-                for (int kb = 0; kb < nk; ++kb, ++g) {
-                    const int st = g % Cfg::STAGES;
-                    ok = mbar_wait_bounded(full(st), (g / Cfg::STAGES) & 1, abort_flag,
-                                           &g_linear_status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t sa = sbase + st * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
+        // The whole warp walks this code and one elected lane issues, so that the descriptors
+        // stay in uniform registers.
+        constexpr uint32_t IDESC = f16_idesc(kM, BN, true);
+        const bool leader = elect_one();
+        const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
+        int st = 0, phase = 0, it = 0;
+        for (int t = blockIdx.x; t < a.tiles && !*abort_flag; t += gridDim.x, ++it) {
+            const int ab = it & 1;
+            if (it >= 2) {
+                mbar_wait_uniform(acc_empty(ab), ((it >> 1) - 1) & 1, abort_addr, &g_linear_status);
+                tc_fence_after();
+            }
+            const uint32_t d = tmem + ab * BN;
+            for (int kb = 0; kb < nk; ++kb) {
+                mbar_wait_uniform(full(st), phase, abort_addr, &g_linear_status);
+                tc_fence_after();
+                const uint32_t sa = sbase + st * Cfg::STAGE;
+                const uint64_t ad = sw128_desc(sa, 16, 1024);
+                const uint64_t bd = sw128_desc(sa + Cfg::A_BYTES, 64 * kK * 2, 1024);
+                if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < kK / 16; ++kk)
-                        tc_mma(tmem + ab * BN, sw128_desc(sa + kk * 32, 16, 1024),
-                               sw128_desc(sb + kk * 2048, 64 * kK * 2, 1024), IDESC,
-                               kb > 0 || kk > 0);
+                        tc_mma(d, ad + kk * (32 >> 4), bd + kk * (2048 >> 4), IDESC, kb > 0 || kk > 0);
                     tc_commit(empty(st));
                 }
-                if (!ok) break;
-                tc_commit(acc_full(ab));
+                __syncwarp();
+                if (++st == Cfg::STAGES) st = 0, phase ^= 1;
             }
-            tc_commit(done);  // every product has completed before the CTA frees its memory
+            if (leader) tc_commit(acc_full(ab));
+            __syncwarp();
+        }
+        if (leader) {  // every product has completed before the CTA frees its memory
+            tc_commit(done);
             mbar_drain(done, 0);
         }
+        __syncwarp();
     } else {
         const int et = tid - 64, quarter = warp & 3;
         const int r = quarter * 32 + lane;  // this thread's row of the tile (its lane)

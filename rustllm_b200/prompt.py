@@ -15,19 +15,38 @@ import torch
 
 from . import _lib
 from ._lib import PagedKV, call
-from .attention import _row_stride
-from .tensor_ops import dtype_code, on_device, stream_ptr
+from .tensor_ops import dtype_code
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "swiglu": 4}
 
 
+_fns: dict = {}
+
+
 def _call(device: torch.device, name: str, *args) -> None:
-    """The C call on the current stream of ``device``, with that device current."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream_ptr(device))
-        return
-    with torch.cuda.device(device):
-        call(name, *args, stream_ptr(device))
+    """The C call on the current stream of ``device``, with that device current.  (A packed
+    layer makes several calls a layer and token: what wraps them is kept to microseconds.)"""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.load(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def _on(device: torch.device, *ts) -> None:
+    """Every given tensor lives on ``device``, a CUDA device: a host or foreign-device pointer
+    must never reach a kernel."""
+    if device.type != "cuda":
+        raise _lib.InvalidArgument(f"tensors must live on a CUDA device, got one on {device}")
+    for t in ts:
+        if t is not None and t.device != device:
+            raise _lib.InvalidArgument(f"tensors must live on {device}, got one on {t.device}")
 
 
 def prompt_status() -> int:
@@ -67,10 +86,14 @@ def _int32(t: torch.Tensor, numel: int | None, what: str) -> None:
 
 
 def _stride(t: torch.Tensor, heads: int, d: int, what: str) -> int:
-    """Row stride of a [rows, heads, D] tensor with packed heads; 0 (packed) for one row, whose
-    stride means nothing."""
-    st = _row_stride(t, heads, d, what)
-    return st if t.shape[0] > 1 else 0
+    """Row stride of a [rows, heads, D] tensor with packed heads (a view into a wider fused
+    projection is fine); 0 (packed) for one row, whose stride means nothing."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != d:
+        raise _lib.ModelFormat(f"{what} must be [rows, {heads}, {d}], got {list(shape)}")
+    if stride[2] != 1 and d > 1 or stride[1] != d and heads > 1:
+        raise _lib.NonContiguousTensor(f"{what} heads must be packed rows of {d} elements")
+    return stride[0] if shape[0] > 1 else 0
 
 
 def batch_tables(kv: PagedKV, new_lens: torch.Tensor, rows: int, *,
@@ -86,7 +109,7 @@ def batch_tables(kv: PagedKV, new_lens: torch.Tensor, rows: int, *,
     the row maps; the rest of them is -1.  Requests that do not fit are refused (their rows
     get -1, ``info[2]`` counts them)."""
     dev = new_lens.device
-    on_device(dev, new_lens, free_blocks, free_start, out)
+    _on(dev, new_lens, free_blocks, free_start, *(out or ()))
     n = kv.num_seqs
     _int32(new_lens, n, "new_lens")
     if free_blocks is not None:
@@ -129,16 +152,18 @@ def rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     place), rotated keys and values to the cache, and the keys to ``k_out`` too when given.
     Returns (q_out, k_out)."""
     dev = q.device
-    on_device(dev, q, k, v, positions, slots, rope, q_out, k_out)
+    cos, sin = rope if rope is not None else (None, None)
+    _on(dev, q, k, v, positions, slots, cos, sin, q_out, k_out)
     if q.dim() != 3:
         raise _lib.ModelFormat(f"q must be [rows, Hq, D], got {list(q.shape)}")
     rows, hq, d = q.shape
     hkv = kv.num_kv_heads
     if d != kv.head_dim:
         raise _lib.ModelFormat(f"the cache holds heads of {kv.head_dim}, got {d}")
-    for t in (q, k, v, q_out, k_out):
-        if t is not None and dtype_code(t.dtype) != kv.dtype:
-            raise _lib.UnsupportedDType("q, k, v and the cache must have one dtype")
+    dtype = q.dtype
+    if dtype_code(dtype) != kv.dtype or any(
+            t is not None and t.dtype != dtype for t in (k, v, q_out, k_out)):
+        raise _lib.UnsupportedDType("q, k, v and the cache must have one dtype")
     qs, ks = _stride(q, hq, d, "q"), _stride(k, hkv, d, "k")
     if _stride(v, hkv, d, "v") != ks:
         raise _lib.NonContiguousTensor("k and v must have the same row stride")
@@ -153,9 +178,7 @@ def rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise _lib.ShapeMismatch("q_out must have q's shape", left=q_out.shape, right=q.shape)
     if k_out is not None and k_out.shape != k.shape:
         raise _lib.ShapeMismatch("k_out must have k's shape", left=k_out.shape, right=k.shape)
-    cos = sin = None
     if rope is not None:
-        cos, sin = rope
         if cos.dtype != torch.float32 or sin.dtype != torch.float32:
             raise _lib.UnsupportedDType("RoPE requires F32 cos/sin tables")
         if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] * 2 != d or not (
@@ -184,7 +207,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
     F32), and lse [rows, Hq] F32 with ``want_lse`` or ``lse``; rows of no sequence are left as
     they are (zeros in new tensors)."""
     dev = q.device
-    on_device(dev, q, k, v, q_start, out, lse)
+    _on(dev, q, k, v, q_start, out, lse)
     if q.dim() != 3 or k.dim() != 3:
         raise _lib.ModelFormat(f"q, k and v must be [rows, heads, D], got {list(q.shape)} and "
                                f"{list(k.shape)}")
@@ -230,7 +253,7 @@ def prompt_linear(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None
     "swiglu" (w = [gate | up] [k, 2n]: silu(gate) * up).  ``residual`` [rows, n] may be ``out``.
     k and n must be multiples of 8, and so must row strides."""
     dev = x.device
-    on_device(dev, x, w, bias, residual, out)
+    _on(dev, x, w, bias, residual, out)
     if x.dim() != 2 or w.dim() != 2:
         raise _lib.ModelFormat(f"Linear expects rank-2 input, got {tuple(x.shape)}")
     try:
