@@ -894,6 +894,24 @@ int make_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, in
     return TMLLM_OK;
 }
 
+int make_store_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows,
+                   int64_t row_bytes) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return fail(TMLLM_DEVICE_ERROR, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+    const cuuint32_t box[2] = {32u, 32u};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(TMLLM_DEVICE_ERROR, "tensor map encoding failed (CUresult %d)",
+                    static_cast<int>(r));
+    return TMLLM_OK;
+}
+
 int make_map_heads(CUtensorMap* map, const void* base, int64_t inner, int64_t heads, int64_t rows,
                    int64_t row_bytes, int box_rows) {
     EncodeTiledFn enc = encode_tiled();

@@ -15,8 +15,8 @@ namespace {
 
 constexpr int kM = 128;        // rows of an output tile (the tensor-memory lanes)
 constexpr int kK = 64;         // K columns per stage: one 128-byte swizzle row
-constexpr int kThreads = 192;  // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
-constexpr int kEpiThreads = 128;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;  // warp 0: TMA, warp 1: MMA, the rest: epilogue
 
 __device__ int g_linear_status;
 
@@ -31,14 +31,24 @@ struct LinArgs {
 };
 
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
-// x Phi(x); through erfc, so the left tail keeps its relative accuracy
-__device__ __forceinline__ float gelu(float x) { return 0.5f * x * erfcf(-0.70710678f * x); }
-__device__ __forceinline__ float activate(float x, int act) {
-    if (act == ACT_RELU) return x > 0.f ? x : (x <= 0.f ? 0.f : x);  // NaN stays
-    if (act == ACT_SILU) return silu(x);
-    if (act == ACT_GELU) return gelu(x);
-    return x;
+// x Phi(x).  Phi(-|x|) = exp(-x^2 / 2) g(|x|): g falls slowly and is fitted by a polynomial in
+// t = 1 / (1 + 0.42 |x| / sqrt 2) (the form Hastings gave for erfc; the coefficients are a
+// least-squares fit reweighted to an even relative error, 1.1e-6 up to |x| = 6.2), so the left
+// tail keeps its relative accuracy.  Two MUFU operations and about 14 others, a third of what
+// erfcf takes.
+__device__ __forceinline__ float gelu(float x) {
+    constexpr float GC0 = 0.11946170f, GC1 = 0.10668742f, GC2 = 0.16564545f, GC3 = -0.05811026f,
+                    GC4 = 0.25197804f, GC5 = -0.08566288f;
+    const float t = __fdividef(1.f, fmaf(0.29698485f, fabsf(x), 1.f));
+    float g = fmaf(t, GC5, GC4);
+    g = fmaf(t, g, GC3);
+    g = fmaf(t, g, GC2);
+    g = fmaf(t, g, GC1);
+    g = fmaf(t, g, GC0) * t;
+    const float tail = __expf(-0.5f * x * x) * g;
+    return x * (x < 0.f ? tail : 1.f - tail);
 }
+__device__ __forceinline__ float relu(float x) { return x > 0.f ? x : (x <= 0.f ? 0.f : x); }  // NaN stays
 
 // BN: accumulator columns of a tile; with GATED half of them are gate and half up columns.
 template <int BN, bool GATED>
@@ -47,13 +57,14 @@ struct LinCfg {
     static constexpr int A_BYTES = kM * kK * 2;
     static constexpr int B_BYTES = BN * kK * 2;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 256 ? 4 : 6;
-    static constexpr int OUT_BYTES = kM * 64 * 2;  // staging: 64 output columns
+    static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
+    // output staging: every epilogue warp has two buffers of 32 rows x 32 columns
     static constexpr int OFF_OUT = STAGES * STAGE;
-    static constexpr int OFF_BIAS = OFF_OUT + 2 * OUT_BYTES;
+    static constexpr int OFF_BIAS = OFF_OUT + kEpiWarps * 2 * 2048;
     static constexpr int OFF_BAR = OFF_BIAS + 2 * BN * 2;  // bias as F16
     static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment
-    static constexpr int TMEM_COLS = 2 * BN;           // two accumulators
+    static constexpr int ACC = BN <= 64 ? 64 : BN <= 128 ? 128 : 256;  // columns apart
+    static constexpr int TMEM_COLS = 2 * ACC;                          // two accumulators
     static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 };
 
@@ -95,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full(i), 1);
-            mbar_init(acc_empty(i), kEpiThreads);
+            mbar_init(acc_empty(i), kEpiWarps);
         }
         mbar_init(done, 1);
         *abort_flag = 0;
@@ -155,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_wait_uniform(acc_empty(ab), ((it >> 1) - 1) & 1, abort_addr, &g_linear_status);
                 tc_fence_after();
             }
-            const uint32_t d = tmem + ab * BN;
+            const uint32_t d = tmem + ab * Cfg::ACC;
             for (int kb = 0; kb < nk; ++kb) {
                 mbar_wait_uniform(full(st), phase, abort_addr, &g_linear_status);
                 tc_fence_after();
@@ -180,93 +191,109 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else {
-        const int et = tid - 64, quarter = warp & 3;
+        // ---- epilogue: a warp owns 32 rows and every other 32 columns of the tile.  It works
+        // alone: its rows leave through its own buffers and bulk stores, the residual of the
+        // next 32 columns is on its way while these are computed.
+        const int quarter = warp & 3, part = (warp - 2) >> 2;
         const int r = quarter * 32 + lane;  // this thread's row of the tile (its lane)
         __half* bias_s = reinterpret_cast<__half*>(smem + Cfg::OFF_BIAS);
+        unsigned char* stage = smem + Cfg::OFF_OUT + (warp - 2) * 4096;
+        const uint32_t stage_addr = smem_u32(stage);
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
         int it = 0, ob = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; t < a.tiles; t += gridDim.x, ++it) {
+        for (int t = blockIdx.x; t < a.tiles && !*abort_flag; t += gridDim.x, ++it) {
             int m, n;
             tile_of(a, t, m, n);
             const int ab = it & 1;
             __half* bias = bias_s + ab * BN;
             if (a.bias) {
-                for (int c = et; c < BN; c += kEpiThreads) {
+                for (int c = tid - 64; c < BN; c += 32 * kEpiWarps) {
                     const int col = GATED ? n * Cfg::ON + c % Cfg::ON : n * BN + c;
                     const bool in = col < a.n;
                     bias[c] = in ? a.bias[GATED && c >= Cfg::ON ? a.n + col : col] : __half(0.f);
                 }
-                named_barrier(1, kEpiThreads);
+                named_barrier(1, 32 * kEpiWarps);
             }
-            ok = mbar_wait_bounded(acc_full(ab), (it >> 1) & 1, abort_flag, &g_linear_status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
             const int64_t row = static_cast<int64_t>(m) * kM + r;
             const bool live = row < a.rows;
+            uint4 res[4];
+            auto load_res = [&](int c0) {
+                const int col = n * Cfg::ON + c0;
+                const __half* p = a.residual + row * a.ld_res + col;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    res[j] = live && c0 < Cfg::ON && col + 8 * j < a.n
+                                 ? *reinterpret_cast<const uint4*>(p + 8 * j)
+                                 : make_uint4(0u, 0u, 0u, 0u);
+            };
+            if (a.residual) load_res(part * 32);
+            mbar_wait_uniform(acc_full(ab), (it >> 1) & 1, abort_addr, &g_linear_status);
+            tc_fence_after();
+            const uint32_t acc = tmem + ab * Cfg::ACC + lane_base;
 #pragma unroll 1
-            for (int c0 = 0; c0 < Cfg::ON; c0 += 64, ob ^= 1) {
+            for (int c0 = part * 32; c0 < Cfg::ON; c0 += 64, ob ^= 1) {
                 const int col0 = n * Cfg::ON + c0;
                 if (col0 >= a.n) break;  // uniform: the rest of the tile is outside
-                // the staging buffer of two chunks ago has been read
-                if (et == 0) bulk_wait_read<1>();
-                named_barrier(1, kEpiThreads);
-                unsigned char* srow = smem + Cfg::OFF_OUT + ob * Cfg::OUT_BYTES + r * 128;
+                float y[32];
+                tmem_ld32(acc + c0, y);
+                if (a.bias) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int cc = c0 + hf * 32;
-                    float y[32];
-                    tmem_ld32(tmem + ab * BN + cc + lane_base, y);
+                    for (int i = 0; i < 32; ++i) y[i] += __half2float(bias[c0 + i]);
+                }
+                if (GATED) {
+                    float u[32];
+                    tmem_ld32(acc + Cfg::ON + c0, u);
                     if (a.bias) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] += __half2float(bias[cc + i]);
-                    }
-                    if (GATED) {
-                        float u[32];
-                        tmem_ld32(tmem + ab * BN + Cfg::ON + cc + lane_base, u);
-                        if (a.bias) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) u[i] += __half2float(bias[Cfg::ON + cc + i]);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = silu(y[i]) * u[i];
-                    } else if (a.act != ACT_NONE) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = activate(y[i], a.act);
-                    }
-                    if (a.residual && live) {
-                        const __half* res = a.residual + row * a.ld_res + n * Cfg::ON + cc;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (n * Cfg::ON + cc + 8 * j >= a.n) break;
-                            const uint4 v = *reinterpret_cast<const uint4*>(res + 8 * j);
-                            float f[8];
-                            Chunk<__half>::unpack(v, f);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) y[8 * j + e] += f[e];
-                        }
+                        for (int i = 0; i < 32; ++i) u[i] += __half2float(bias[Cfg::ON + c0 + i]);
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *reinterpret_cast<uint4*>(srow + (((hf * 4 + j) ^ (r & 7)) << 4)) =
-                            make_uint4(pack_half2(y[8 * j], y[8 * j + 1]),
-                                       pack_half2(y[8 * j + 2], y[8 * j + 3]),
-                                       pack_half2(y[8 * j + 4], y[8 * j + 5]),
-                                       pack_half2(y[8 * j + 6], y[8 * j + 7]));
+                    for (int i = 0; i < 32; ++i) y[i] = silu(y[i]) * u[i];
+                } else if (a.act == ACT_GELU) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = gelu(y[i]);
+                } else if (a.act == ACT_SILU) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = silu(y[i]);
+                } else if (a.act == ACT_RELU) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = relu(y[i]);
                 }
+                if (a.residual) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float f[8];
+                        Chunk<__half>::unpack(res[j], f);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[8 * j + e] += f[e];
+                    }
+                    load_res(c0 + 64);
+                }
+                // the buffer of two stores ago has been read
+                if (lane == 0) bulk_wait_read<1>();
+                __syncwarp();
+                unsigned char* srow = stage + ob * 2048 + lane * 64;  // 64-byte swizzle
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<uint4*>(srow + ((j ^ (lane >> 1 & 3)) << 4)) =
+                        make_uint4(pack_half2(y[8 * j], y[8 * j + 1]),
+                                   pack_half2(y[8 * j + 2], y[8 * j + 3]),
+                                   pack_half2(y[8 * j + 4], y[8 * j + 5]),
+                                   pack_half2(y[8 * j + 6], y[8 * j + 7]));
                 fence_async_smem();
-                named_barrier(1, kEpiThreads);
-                if (et == 0) {
-                    tma_store_2d(&omap, col0, m * kM,
-                                 sbase + Cfg::OFF_OUT + ob * Cfg::OUT_BYTES);
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_2d(&omap, col0, m * kM + quarter * 32, stage_addr + ob * 2048);
                     bulk_commit();
                 }
             }
             tc_fence_before();
-            mbar_arrive(acc_empty(ab));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty(ab));
         }
-        if (et == 0) bulk_wait<0>();
+        if (lane == 0) bulk_wait<0>();
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
@@ -278,6 +305,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// Waves of the grid times the cost of a tile: BN columns take BN / 2 cycles of the tensor cores a K
+// step of 16, and below 128 columns A's 4 KB bound the step by shared memory instead; the constant
+// is what a tile costs beside its products (measured: see choose()).
+inline int64_t cost_of(int64_t m_tiles, int64_t n_tiles, int bn, int64_t ksteps) {
+    const int64_t waves = (m_tiles * n_tiles + device_sm_count() - 1) / device_sm_count();
+    return waves * ((bn > 128 ? bn : 64 + bn / 2) * ksteps + 1500);
+}
+
 template <int BN, bool GATED>
 int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ldo,
            LinArgs a, cudaStream_t s) {
@@ -286,7 +321,7 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, in
     if (int st = make_map(&xmap, x, a.k, a.rows, ldx * 2, kM)) return st;
     if (int st = make_map(&wmap, w, GATED ? 2 * static_cast<int64_t>(a.n) : a.n, a.k, ldw * 2, kK))
         return st;
-    if (int st = make_map(&omap, out, a.n, a.rows, ldo * 2, kM)) return st;
+    if (int st = make_store_map(&omap, out, a.n, a.rows, ldo * 2)) return st;
     a.m_tiles = (a.rows + kM - 1) / kM;
     a.n_tiles = (a.n + Cfg::ON - 1) / Cfg::ON;
     int64_t tiles;
@@ -367,8 +402,22 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     a.n = n;
     a.act = activation;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (activation == ACT_SWIGLU) return launch<256, true>(x, ldx, w, ldw, out, ldo, a, s);
-    return launch<256, false>(x, ldx, w, ldw, out, ldo, a, s);
+    const int64_t mt = (rows + kM - 1) / kM, ksteps = (k + 15) / 16;
+    auto tiles = [&](int on) { return (static_cast<int64_t>(n) + on - 1) / on; };
+    if (activation == ACT_SWIGLU) {
+        const bool wide_tile = cost_of(mt, tiles(128), 256, ksteps) <= cost_of(mt, tiles(64), 128, ksteps);
+        return wide_tile ? launch<256, true>(x, ldx, w, ldw, out, ldo, a, s)
+                         : launch<128, true>(x, ldx, w, ldw, out, ldo, a, s);
+    }
+    int best = 256;
+    for (int bn : {192, 128, 64})
+        if (cost_of(mt, tiles(bn), bn, ksteps) < cost_of(mt, tiles(best), best, ksteps)) best = bn;
+    switch (best) {
+        case 64: return launch<64, false>(x, ldx, w, ldw, out, ldo, a, s);
+        case 128: return launch<128, false>(x, ldx, w, ldw, out, ldo, a, s);
+        case 192: return launch<192, false>(x, ldx, w, ldw, out, ldo, a, s);
+        default: return launch<256, false>(x, ldx, w, ldw, out, ldo, a, s);
+    }
 }
 
 }  // extern "C"

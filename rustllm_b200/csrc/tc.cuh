@@ -19,6 +19,10 @@ namespace tmllm {
 int make_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t row_bytes,
              int box_rows, bool f32 = false);
 
+// For stores from buffers of 32 rows x 32 F16 columns in the 64-byte swizzle (chunk c of row r at
+// chunk c ^ (r / 2 % 4)).
+int make_store_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows,
+                   int64_t row_bytes);
 // The same over [rows][heads][inner] F16 tensors (heads `inner` elements apart, rows
 // `row_bytes` apart): boxes of 64 columns of one head x box_rows rows.  Columns past `inner`
 // read zeros, also where the next head's lie.
