@@ -16,8 +16,9 @@ into the projection that produces it, so a layer is five launches:
     x -> [norm + QKV] -> attention -> [O + residual -> x] -> [norm + gate/up + SwiGLU]
       -> [down + residual -> x]
 
-Prompts and larger batches use plain cuBLAS GEMMs (torch.matmul) between the norm, SwiGLU
-and attention kernels.  With up to 16 sequences (F16) the step ends in one launch: the final
+Prompts of one length (``prefill``) and larger batches use plain cuBLAS GEMMs (torch.matmul)
+between the norm, SwiGLU and attention kernels; prompts of different lengths run packed
+(``prefill_packed``) through ``prompt_linear``, ``rope_append`` and ``prompt_attention``.  With up to 16 sequences (F16) the step ends in one launch: the final
 RMSNorm, the vocabulary head and the greedy pick (``lm_head``, tmllm_lm_head); larger
 batches use a cuBLAS head between the norm and argmax kernels.  Weights keep the
 reference's [in, out] layout (src/nn/linear.rs:26-27); Q, K, V and gate/up are concatenated
@@ -520,6 +521,69 @@ class Decoder:
         self.x.copy_(x.index_select(0, last))
         self._head(down.index_select(0, last))
         self.cache.advance(S)
+        return self.next_ids.clone()
+
+    def prefill_packed(self, prompts) -> torch.Tensor:
+        """``prefill`` for prompts of different lengths: ``prompts`` holds one rank-1 id tensor
+        per sequence (at least one token each), packed back to back, so no row is padding.
+        Row maps come from ``batch_tables``, the projections with bias-free residual / SwiGLU
+        epilogues from ``prompt_linear``, and ``rope_append`` fills the cache; whole prompts
+        attend by ``prompt_attention``, prompts behind cached tokens by ``gqa_prefill``.
+        Advances every length by its prompt's and returns the greedy token after each prompt
+        (logits of its last row, ``self.logits``).  F16 models with dimensions in multiples
+        of 8."""
+        from .attention import gqa_prefill
+        from .prompt import batch_tables, prompt_attention, prompt_linear, rope_append
+        cfg, w = self.cfg, self.w
+        if self.dtype != torch.float16:
+            raise _lib.UnsupportedDType(f"prefill_packed takes F16 models, got {self.dtype}")
+        if len(prompts) != self.B:
+            raise _lib.ShapeMismatch(f"prefill_packed expects {self.B} prompts, got "
+                                     f"{len(prompts)}", left=[self.B], right=[len(prompts)])
+        lens = [int(p.numel()) for p in prompts]
+        if any(p.dim() != 1 for p in prompts) or min(lens) == 0:
+            raise _lib.InvalidShape("every prompt must be a rank-1 tensor of at least one token id")
+        cached = self.cache.lens()
+        for c, n in zip(cached, lens):
+            if c + n > self.max_seq_len:
+                raise _lib.PositionOutOfRange(start_pos=c, seq_len=n, max_seq_len=self.max_seq_len)
+        ids = torch.cat([p.to(device=self.device, dtype=torch.int64) for p in prompts])
+        self.check_ids(ids)
+        ids = ids.to(torch.int32)
+        T, h, d = sum(lens), cfg.hidden_size, cfg.head_dim
+        hq, hkv = cfg.num_heads, cfg.num_kv_heads
+        for s, n in enumerate(lens):
+            self.cache.reserve(s, n)
+        new = torch.tensor(lens, dtype=torch.int32, device=self.device)
+        maps = batch_tables(self.cache.view(0), new, T)
+        e = dict(dtype=self.dtype, device=self.device)
+        x, hn = torch.empty((T, h), **e), torch.empty((T, h), **e)
+        qkv = torch.empty((T, (hq + 2 * hkv) * d), **e)
+        attn = torch.empty((T, hq, d), **e)
+        act = torch.empty((T, cfg.intermediate_size), **e)
+        q = qkv[:, :hq * d].view(T, hq, d)
+        k = qkv[:, hq * d:(hq + hkv) * d].view(T, hkv, d)
+        v = qkv[:, (hq + hkv) * d:].view(T, hkv, d)
+        call("tmllm_embedding", self.dt, w.embedding.data_ptr(), ids.data_ptr(), x.data_ptr(), T,
+             h, cfg.vocab_size, self.bad.data_ptr(), stream_ptr(self.device))
+        for li, L in enumerate(w.layers):
+            kv = self.cache.view(li)
+            self._norm(x, None, L["attn_norm"], hn, None)
+            prompt_linear(hn, L["wqkv"], out=qkv)
+            rope_append(kv, q, k, v, maps.positions, maps.slots, rope=self.rope, q_out=q, k_out=k)
+            if any(cached):
+                gqa_prefill(kv, q, None, None, q_start=maps.q_start, max_rows=max(lens), out=attn)
+            else:
+                prompt_attention(q, k, v, maps.q_start, max(lens), out=attn)
+            prompt_linear(attn.view(T, -1), L["wo"], residual=x, out=x)
+            self._norm(x, None, L["mlp_norm"], hn, None)
+            prompt_linear(hn, L["wgu"], activation="swiglu", out=act)
+            prompt_linear(act, L["wd"], residual=x, out=x)
+        # only each prompt's last row reaches the head
+        self.x.copy_(x.index_select(0, maps.q_start[1:] - 1))
+        self._head(None)
+        for s, n in enumerate(lens):
+            self.cache.advance(n, s)
         return self.next_ids.clone()
 
     def prefill_stepwise(self, prompts: torch.Tensor) -> torch.Tensor:

@@ -590,3 +590,81 @@ def test_two_streams_at_once(cuda):
     torch.cuda.synchronize()
     for j, y in zip(jobs, alone):
         assert torch.equal(j[-1]["y"], y)
+
+
+# ---- the decoder's packed prefill -------------------------------------------------------
+def packed_decoder(dev, seqs, seed=3, hidden=256, heads=4, kv=2, inter=512, max_len=400):
+    from rustllm_b200.decoder import Decoder, DecoderWeights, ModelConfig
+    cfg = ModelConfig(vocab_size=1000, hidden_size=hidden, intermediate_size=inter, num_layers=2,
+                      num_heads=heads, num_kv_heads=kv, max_seq_len=max_len, rms_norm_eps=1e-5,
+                      rope_theta=10000.0)
+    w = DecoderWeights(cfg, device=dev, seed=seed, std=0.05)
+    return cfg, w, Decoder(cfg, w, seqs, device=dev, shuffle_seed=7)
+
+
+def prompt_ids(dev, lens, seed=0):
+    g = gen(dev, seed)
+    return [torch.randint(0, 1000, (n,), generator=g, device=dev) for n in lens]
+
+
+def close_logits(got, want):
+    """A few F16 layers against another order of the same roundings (as the decoder's own
+    tests): 3e-2 of the largest logit."""
+    got, want = got.double(), want.double()
+    assert float((got - want).abs().max()) <= 3e-2 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("lens,hidden,heads,kv", [([37, 1, 200, 16], 256, 4, 2),
+                                                  ([5, 130], 576, 9, 3), ([300], 512, 4, 4)])
+def test_decoder_prefill_packed(cuda, lens, hidden, heads, kv):
+    """Logits after ragged prompts against the float32 model, the cache and decode steps behind
+    them against prompts run token by token."""
+    from model_reference import reference_forward
+    cfg, w, dec = packed_decoder(cuda, len(lens), hidden=hidden, heads=heads, kv=kv)
+    prompts = prompt_ids(cuda, lens)
+    first = dec.prefill_packed(prompts)
+    assert dec.cache.lens() == lens and rb.prompt_status() == 0
+    for s, p in enumerate(prompts):
+        close_logits(dec.logits[s], reference_forward(cfg, w, p)[-1])
+    assert torch.equal(first, dec.next_ids)
+    tokens = dec.decode(3, first)
+    # the same prompts one sequence at a time, through the equal-length prefill
+    for s, p in enumerate(prompts):
+        _, _, one = packed_decoder(cuda, 1, hidden=hidden, heads=heads, kv=kv)
+        one.prefill(p[None])
+        for li in range(cfg.num_layers):
+            for a, b in zip(dec.cache.gather(li, s), one.cache.gather(li, 0)):
+                n = lens[s]
+                err = (a[:, :n].double() - b[:, :n].double()).abs().max()
+                assert float(err) <= 2e-2 * float(b.double().abs().max())
+    # and the steps behind them follow the full model on prompt + tokens
+    full = torch.cat([prompts[0], torch.stack([first[0], *tokens[:2, 0]]).long()])
+    close_logits(dec.logits[0], reference_forward(cfg, w, full)[-1])
+
+
+def test_decoder_prefill_packed_behind_cached_tokens(cuda):
+    """A second ragged batch attends what the first one cached (the paged path)."""
+    from model_reference import reference_forward
+    cfg, w, dec = packed_decoder(cuda, 3)
+    a, b = prompt_ids(cuda, [20, 3, 150], 1), prompt_ids(cuda, [1, 140, 30], 2)
+    dec.prefill_packed(a)
+    dec.prefill_packed(b)
+    assert dec.cache.lens() == [21, 143, 180]
+    for s in range(3):
+        close_logits(dec.logits[s], reference_forward(cfg, w, torch.cat([a[s], b[s]]))[-1])
+
+
+def test_decoder_prefill_packed_refusals(cuda):
+    _, _, dec = packed_decoder(cuda, 2, max_len=32)
+    ids = prompt_ids(cuda, [3, 4])
+    with pytest.raises(rb.ShapeMismatch):
+        dec.prefill_packed(ids[:1])
+    with pytest.raises(rb.InvalidShape):
+        dec.prefill_packed([ids[0], ids[1][:0]])
+    with pytest.raises(rb.InvalidShape):
+        dec.prefill_packed([ids[0], ids[1][None]])
+    with pytest.raises(rb.PositionOutOfRange):
+        dec.prefill_packed([ids[0], torch.zeros(33, dtype=torch.int64, device=cuda)])
+    with pytest.raises(rb.InvalidArgument):
+        dec.prefill_packed([ids[0], torch.full((2,), 1000, device=cuda)])
+    assert dec.cache.lens() == [0, 0]
