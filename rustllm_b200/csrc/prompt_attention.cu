@@ -47,26 +47,40 @@ __device__ __forceinline__ int seq_rows(const PromptArgs& a, int s, int64_t* row
 }
 
 // ---- CUDA-core form: any type and head size up to 256 -----------------------------------
-// One CTA per (64 query rows, query head, sequence), 256 threads; thread (ty, tx) holds rows
-// 4 ty .. 4 ty + 3 of S (columns tx + 16 c) and of O (columns tx + 16 c).  DP: head size
-// rounded up to 64 / 128 / 256.
-constexpr int kFmaTile = 64;
+// One CTA per (16 RT query rows, query head, sequence), 256 threads; thread (ty, tx) holds RT rows
+// from RT ty on of S (columns tx + 16 c of a tile of 64 keys) and of O (columns 4 tx + 64 c ..).  DP: head size
+// rounded up to 64 / 128 / 256.  Both products run on packed F32 pairs (two multiply-adds an
+// instruction) out of 16-byte shared-memory reads, 64 multiply-adds per 8 reads; with F32 rows
+// on the 16-byte grid the next K and V tiles are copied while this one is computed (DP <= 128).
+// Bound by the F32 multiply-add rate at long prompts, by latency at short ones.
+constexpr int kFmaTile = 64;  // keys
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int row_tiles) {
-    constexpr int LD = DP + 1;  // odd pitch: column walks hit every bank
-    extern __shared__ float fsm[];
-    float* qs = fsm;                       // [64][LD]
-    float* ks = qs + kFmaTile * LD;        // [64][LD]
-    float* vs = ks + kFmaTile * LD;        // [64][DP]
-    float* ps = vs + kFmaTile * DP;        // [64][65]
+template <int DP, int RT>
+struct FmaCfg {
+    static constexpr int ROWS = 16 * RT;
+    static constexpr int LD = DP + 4;  // pitch of Q and K: rows 16 bytes apart in the banks
+    static constexpr int BUFS = DP <= 128 ? 2 : 1;
+    static constexpr int KV = kFmaTile * (LD + DP);  // floats of a K and a V tile
+    static constexpr int LP = kFmaTile + 4;
+    static constexpr int SMEM = (ROWS * LD + BUFS * KV + ROWS * LP) * 4;
+};
+
+template <typename T, int DP, int RT>
+__global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int row_tiles,
+                                                         int async) {
+    using Cfg = FmaCfg<DP, RT>;
+    constexpr int ROWS = Cfg::ROWS, LD = Cfg::LD, LP = Cfg::LP, CG = DP / 64;
+    extern __shared__ __align__(16) float fsm[];
+    float* qs = fsm;                          // [ROWS][LD]
+    float* kv0 = qs + ROWS * LD;              // [BUFS]: K [64][LD], V [64][DP]
+    float* ps = kv0 + Cfg::BUFS * Cfg::KV;    // [ROWS][LP]
     const int64_t hb = static_cast<int64_t>(a.q_heads) * a.num_seqs;
     const int tile = row_tiles - 1 - static_cast<int>(blockIdx.x / hb);
     const int h = static_cast<int>(blockIdx.x % hb) % a.q_heads;
     const int s = static_cast<int>(blockIdx.x % hb) / a.q_heads;
     int64_t row0 = 0;
     const int n = seq_rows(a, s, &row0);
-    const int q_lo = tile * kFmaTile;
+    const int q_lo = tile * ROWS;
     if (q_lo >= n) return;
     const int kvh = h / a.group, D = a.head_dim;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -74,49 +88,95 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
                   static_cast<int64_t>(h) * D;
     const T* kg = static_cast<const T*>(a.k) + row0 * a.kv_stride + static_cast<int64_t>(kvh) * D;
     const T* vg = static_cast<const T*>(a.v) + row0 * a.kv_stride + static_cast<int64_t>(kvh) * D;
-    for (int i = tid; i < kFmaTile * DP; i += 256) {
+    const int q_hi = q_lo + ROWS < n ? q_lo + ROWS : n;  // keys [0, q_hi) are visible
+    // rows j0 .. of K and V (zeros past the last visible key and the head size)
+    auto load = [&](int j0, int buf) {
+        float* ks = kv0 + buf * Cfg::KV;
+        float* vs = ks + kFmaTile * LD;
+        if (async) {
+            for (int i = tid; i < kFmaTile * (DP / 4); i += 256) {
+                const int r = i / (DP / 4), c = (i % (DP / 4)) * 4;
+                const bool in = j0 + r < q_hi && c < D;  // D is a multiple of 4 here
+                const int64_t off = in ? static_cast<int64_t>(j0 + r) * a.kv_stride + c : 0;
+                cp_async16(ks + r * LD + c, kg + off, in ? 16 : 0);
+                cp_async16(vs + r * DP + c, vg + off, in ? 16 : 0);
+            }
+            cp_async_commit();
+        } else {
+            for (int i = tid; i < kFmaTile * DP; i += 256) {
+                const int r = i / DP, c = i % DP;
+                const bool in = j0 + r < q_hi && c < D;
+                const int64_t off = static_cast<int64_t>(j0 + r) * a.kv_stride + c;
+                ks[r * LD + c] = in ? to_f32<T>(kg[off]) : 0.f;
+                vs[r * DP + c] = in ? to_f32<T>(vg[off]) : 0.f;
+            }
+        }
+    };
+    load(0, 0);
+    for (int i = tid; i < ROWS * DP; i += 256) {
         const int r = i / DP, c = i % DP;
         qs[r * LD + c] = (q_lo + r < n && c < D) ? to_f32<T>(qg[r * a.q_stride + c]) : 0.f;
     }
-    float o[4][DP / 16], m[4], l[4];
+    float2 o[RT][2 * CG];
+    float m[RT], l[RT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RT; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) o[i][c] = 0.f;
+        for (int c = 0; c < 2 * CG; ++c) o[i][c] = make_float2(0.f, 0.f);
     }
-    const int q_hi = q_lo + kFmaTile < n ? q_lo + kFmaTile : n;  // keys [0, q_hi) are visible
+    int buf = 0;
     for (int j0 = 0; j0 < q_hi; j0 += kFmaTile) {
-        __syncthreads();
-        for (int i = tid; i < kFmaTile * DP; i += 256) {
-            const int r = i / DP, c = i % DP;
-            const bool in = j0 + r < q_hi && c < D;
-            const int64_t off = static_cast<int64_t>(j0 + r) * a.kv_stride + c;
-            ks[r * LD + c] = in ? to_f32<T>(kg[off]) : 0.f;
-            vs[r * DP + c] = in ? to_f32<T>(vg[off]) : 0.f;
+        const bool ahead = Cfg::BUFS == 2 && async && j0 + kFmaTile < q_hi;
+        if (ahead) {
+            load(j0 + kFmaTile, buf ^ 1);
+            cp_async_wait<1>();
+        } else {
+            cp_async_wait<0>();
         }
         __syncthreads();
-        float sc[4][4] = {};
-        for (int d = 0; d < D; ++d) {
-            float qv[4], kv[4];
+        const float* ks = kv0 + buf * Cfg::KV;
+        const float* vs = ks + kFmaTile * LD;
+        const bool diag = j0 + kFmaTile > q_lo;
+        // 0 * inf is not 0: a diagonal tile with non-finite values takes the masked product
+        bool odd = false;
+        if (diag) {
+            for (int i = tid; i < kFmaTile * DP; i += 256) odd |= !(fabsf(vs[i]) < INFINITY);
+            odd = __syncthreads_or(odd);
+        }
+        float2 s2[RT][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) qv[i] = qs[(4 * ty + i) * LD + d];
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) kv[c] = ks[(tx + 16 * c) * LD + d];
+            for (int c = 0; c < 4; ++c) s2[i][c] = make_float2(0.f, 0.f);
+#pragma unroll 4
+        for (int d = 0; d < D; d += 4) {  // rows are zero past D
+            float4 qv[RT], kv[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < RT; ++i)
+                qv[i] = *reinterpret_cast<const float4*>(qs + (RT * ty + i) * LD + d);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) sc[i][c] = fmaf(qv[i], kv[c], sc[i][c]);
+            for (int c = 0; c < 4; ++c)
+                kv[c] = *reinterpret_cast<const float4*>(ks + (tx + 16 * c) * LD + d);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    s2[i][c] = __ffma2_rn(make_float2(qv[i].x, qv[i].y),
+                                          make_float2(kv[c].x, kv[c].y), s2[i][c]);
+                    s2[i][c] = __ffma2_rn(make_float2(qv[i].z, qv[i].w),
+                                          make_float2(kv[c].z, kv[c].w), s2[i][c]);
+                }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int qi = q_lo + 4 * ty + i;
-            float mt = -INFINITY;
+        for (int i = 0; i < RT; ++i) {
+            const int qi = q_lo + RT * ty + i;
+            float sc[4], mt = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                sc[i][c] = j0 + tx + 16 * c <= qi ? sc[i][c] * a.scale_log2 : -INFINITY;
-                mt = fmaxf(mt, sc[i][c]);
+                sc[c] = j0 + tx + 16 * c <= qi ? (s2[i][c].x + s2[i][c].y) * a.scale_log2 : -INFINITY;
+                mt = fmaxf(mt, sc[c]);
             }
 #pragma unroll
             for (int w = 8; w > 0; w >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, w));
@@ -126,8 +186,8 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
             float ls = 0.f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const float p = exp2f(sc[i][c] - base);
-                ps[(4 * ty + i) * 65 + tx + 16 * c] = p;
+                const float p = exp2f(sc[c] - base);
+                ps[(RT * ty + i) * LP + tx + 16 * c] = p;
                 ls += p;
             }
 #pragma unroll
@@ -135,55 +195,105 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
             l[i] = l[i] * corr + ls;
             m[i] = mn;
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) o[i][c] *= corr;
+            for (int c = 0; c < 2 * CG; ++c)
+                o[i][c] = make_float2(o[i][c].x * corr, o[i][c].y * corr);
         }
         __syncwarp();  // the rows of ps a warp reads are the ones its own lanes wrote
-        const int nk = q_hi - j0 < kFmaTile ? q_hi - j0 : kFmaTile;
-        const bool diag = j0 + nk - 1 > q_lo;
-        for (int j = 0; j < nk; ++j) {
-            float pv[4];
+        if (!odd) {
+#pragma unroll 2
+            for (int j = 0; j < kFmaTile; j += 4) {  // P is zero for keys that are not there
+                float4 pv[RT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pv[i] = ps[(4 * ty + i) * 65 + j];
+                for (int i = 0; i < RT; ++i)
+                    pv[i] = *reinterpret_cast<const float4*>(ps + (RT * ty + i) * LP + j);
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) {
-                const float vv = vs[j * DP + tx + 16 * c];
+                for (int c = 0; c < CG; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)  // a masked value must not reach a sum (0 * inf)
-                    if (!diag || j0 + j <= q_lo + 4 * ty + i) o[i][c] = fmaf(pv[i], vv, o[i][c]);
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 vv =
+                            *reinterpret_cast<const float4*>(vs + (j + e) * DP + 64 * c + 4 * tx);
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            const float p = e == 0 ? pv[i].x : e == 1 ? pv[i].y : e == 2 ? pv[i].z : pv[i].w;
+                            const float2 p2 = make_float2(p, p);
+                            o[i][2 * c] = __ffma2_rn(p2, make_float2(vv.x, vv.y), o[i][2 * c]);
+                            o[i][2 * c + 1] = __ffma2_rn(p2, make_float2(vv.z, vv.w), o[i][2 * c + 1]);
+                        }
+                    }
             }
+        } else {
+            const int nk = q_hi - j0 < kFmaTile ? q_hi - j0 : kFmaTile;
+            for (int j = 0; j < nk; ++j)
+                for (int i = 0; i < RT; ++i) {
+                    if (j0 + j > q_lo + RT * ty + i) continue;
+                    const float p = ps[(RT * ty + i) * LP + j];
+#pragma unroll
+                    for (int c = 0; c < CG; ++c) {
+                        const float* vv = vs + j * DP + 64 * c + 4 * tx;
+                        o[i][2 * c].x = fmaf(p, vv[0], o[i][2 * c].x);
+                        o[i][2 * c].y = fmaf(p, vv[1], o[i][2 * c].y);
+                        o[i][2 * c + 1].x = fmaf(p, vv[2], o[i][2 * c + 1].x);
+                        o[i][2 * c + 1].y = fmaf(p, vv[3], o[i][2 * c + 1].y);
+                    }
+                }
+        }
+        __syncthreads();  // the tiles are done with
+        if (ahead) {
+            buf ^= 1;
+        } else if (j0 + kFmaTile < q_hi) {
+            load(j0 + kFmaTile, buf);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = q_lo + 4 * ty + i;
+    for (int i = 0; i < RT; ++i) {
+        const int r = q_lo + RT * ty + i;
         if (r >= n) continue;
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];  // every score -inf: zeros
         const int64_t off = (row0 + r) * a.out_stride + static_cast<int64_t>(h) * D;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) {
-            const int d = tx + 16 * c;
-            if (d >= D) continue;
-            if (a.out_f32) static_cast<float*>(a.out)[off + d] = o[i][c] * inv;
-            else static_cast<T*>(a.out)[off + d] = from_f32<T>(o[i][c] * inv);
-        }
+        for (int c = 0; c < CG; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 64 * c + 4 * tx + e;
+                if (d >= D) continue;
+                const float2 x = o[i][2 * c + (e >> 1)];
+                const float y = ((e & 1) ? x.y : x.x) * inv;
+                if (a.out_f32) static_cast<float*>(a.out)[off + d] = y;
+                else static_cast<T*>(a.out)[off + d] = from_f32<T>(y);
+            }
         if (a.lse && tx == 0)
-            a.lse[(row0 + r) * a.q_heads + h] = (m[i] + log2f(l[i])) * kLn2;
+            a.lse[(row0 + r) * a.q_heads + h] =
+                ((m[i] == -INFINITY ? 0.f : m[i]) + log2f(l[i])) * kLn2;
     }
 }
 
-template <typename T, int DP>
-int launch_fma(const PromptArgs& a, cudaStream_t s) {
-    const int row_tiles = (a.max_rows + kFmaTile - 1) / kFmaTile;
+template <typename T, int DP, int RT>
+int launch_fma_rows(const PromptArgs& a, cudaStream_t s) {
+    const int row_tiles = (a.max_rows + 16 * RT - 1) / (16 * RT);
     int64_t ctas;
     if (!mul_ok(static_cast<int64_t>(row_tiles) * a.q_heads, a.num_seqs, &ctas) ||
         ctas > INT32_MAX)
         return fail(TMLLM_INVALID_SHAPE, "too many prompt tiles");
-    constexpr int smem = (2 * kFmaTile * (DP + 1) + kFmaTile * DP + kFmaTile * 65) * 4;
-    TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_fma_kernel<T, DP>,
+    constexpr int smem = FmaCfg<DP, RT>::SMEM;
+    static_assert(smem <= 227 * 1024, "shared memory of one CTA");
+    const int async = sizeof(T) == 4 && a.head_dim % 4 == 0 && a.kv_stride % 4 == 0 &&
+                      aligned16(a.k) && aligned16(a.v);
+    TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_fma_kernel<T, DP, RT>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    prompt_fma_kernel<T, DP><<<static_cast<unsigned>(ctas), 256, smem, s>>>(a, row_tiles);
+    prompt_fma_kernel<T, DP, RT><<<static_cast<unsigned>(ctas), 256, smem, s>>>(a, row_tiles, async);
     TMLLM_LAUNCH_TRY();
     return TMLLM_OK;
+}
+
+// 64 query rows a CTA read K and V half as often; 32 spread a small batch over more SMs and halve
+// its longest CTA (F32, 270 CTAs of 64 rows over 9 prompts of up to 500 tokens: 53 us against 45;
+// 420 CTAs over 4 x 500 tokens, 12 heads of 64: 81 against 104; 4096 tokens, 8 / 2 heads of 128:
+// 957 us, 36 TFLOP/s, against 1562).
+template <typename T, int DP>
+int launch_fma(const PromptArgs& a, cudaStream_t s) {
+    const int64_t ctas = (a.rows / 64 + a.num_seqs) * a.q_heads;
+    return ctas < 2 * device_sm_count() ? launch_fma_rows<T, DP, 2>(a, s)
+                                        : launch_fma_rows<T, DP, 4>(a, s);
 }
 
 template <typename T>

@@ -51,11 +51,14 @@ __device__ __forceinline__ float gelu(float x) {
 __device__ __forceinline__ float relu(float x) { return x > 0.f ? x : (x <= 0.f ? 0.f : x); }  // NaN stays
 
 // BN: accumulator columns of a tile; with GATED half of them are gate and half up columns.
-template <int BN, bool GATED>
+// PAIR: the two CTAs of a cluster share a tile of 256 rows, each with its 128 rows of A and half
+// the columns of W in shared memory.
+template <int BN, bool GATED, bool PAIR = false>
 struct LinCfg {
     static constexpr int ON = GATED ? BN / 2 : BN;  // output columns of a tile
     static constexpr int A_BYTES = kM * kK * 2;
-    static constexpr int B_BYTES = BN * kK * 2;
+    static constexpr int BC = PAIR ? BN / 2 : BN;  // columns of W in this CTA
+    static constexpr int B_BYTES = BC * kK * 2;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
     // output staging: every epilogue warp has two buffers of 32 rows x 32 columns
@@ -79,12 +82,12 @@ __device__ __forceinline__ void tile_of(const LinArgs& a, int t, int& m, int& n)
     n = r / gm;
 }
 
-template <int BN, bool GATED>
+template <int BN, bool GATED, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_linear_kernel(const __grid_constant__ CUtensorMap xmap,
                          const __grid_constant__ CUtensorMap wmap,
                          const __grid_constant__ CUtensorMap omap, const LinArgs a) {
-    using Cfg = LinCfg<BN, GATED>;
+    using Cfg = LinCfg<BN, GATED, PAIR>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
@@ -106,22 +109,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full(i), 1);
-            mbar_init(acc_empty(i), kEpiWarps);
+            mbar_init(acc_empty(i), kEpiWarps * (PAIR ? 2 : 1));
         }
         mbar_init(done, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         smem_u32(tmem_slot)),
-                     "r"(Cfg::TMEM_COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_u32(tmem_slot)),
+                         "r"(Cfg::TMEM_COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_u32(tmem_slot)),
+                         "r"(Cfg::TMEM_COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
-    __syncthreads();
+    if (PAIR) cluster_sync_all();  // the other CTA's barriers are ready too
+    else __syncthreads();
     tc_fence_after();
+    // the pair walks the tiles together; this CTA has the rows from `row_of` on
+    const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
+    const int tile_first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+    const int tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    auto row_of = [&](int m) { return PAIR ? (2 * m + rank) * kM : m * kM; };
     const uint32_t tmem = *tmem_slot;
     const int nk = (a.k + kK - 1) / kK;
 
@@ -129,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             int g = 0;
             bool ok = true;
-            for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+            for (int t = tile_first; ok && t < a.tiles; t += tile_step) {
                 int m, n;
                 tile_of(a, t, m, n);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
@@ -139,28 +156,39 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!ok) break;
                     }
                     const uint32_t sa = sbase + st * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
-                    mbar_arrive_tx(full(st), Cfg::STAGE);
-                    tma_load_2d(sa, &xmap, kb * kK, m * kM, full(st));
+                    // both CTAs' copies count on the first one's barrier, where the products wait
+                    if (!PAIR || rank == 0) mbar_arrive_tx(full(st), Cfg::STAGE * (PAIR ? 2 : 1));
+                    const uint32_t fb = PAIR ? cluster_addr(full(st), 0) : full(st);
+                    auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+                        if (PAIR) tma_load_2d_pair(dst, map, x, y, fb);
+                        else tma_load_2d(dst, map, x, y, fb);
+                    };
+                    load(sa, &xmap, kb * kK, row_of(m));
 #pragma unroll
-                    for (int c = 0; c < BN / 64; ++c) {
-                        const int col = GATED ? (c < BN / 128 ? n * Cfg::ON + c * 64
-                                                              : a.n + n * Cfg::ON + (c - BN / 128) * 64)
-                                              : n * BN + c * 64;
-                        tma_load_2d(sb + c * (64 * kK * 2), &wmap, col, kb * kK, full(st));
+                    for (int c = 0; c < Cfg::BC / 64; ++c) {
+                        const int tc = rank * Cfg::BC + c * 64;  // accumulator column
+                        const int col = GATED ? (tc < Cfg::ON ? n * Cfg::ON + tc
+                                                              : a.n + n * Cfg::ON + tc - Cfg::ON)
+                                              : n * BN + tc;
+                        load(sb + c * (64 * kK * 2), &wmap, col, kb * kK);
                     }
                 }
             }
-            for (int i = g < Cfg::STAGES ? 0 : g - Cfg::STAGES; !ok && i < g; ++i)
+            for (int i = g < Cfg::STAGES ? 0 : g - Cfg::STAGES; !ok && rank == 0 && i < g; ++i)
                 mbar_drain(full(i % Cfg::STAGES), (i / Cfg::STAGES) & 1);
         }
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
         // The whole warp walks this code and one elected lane issues, so that the descriptors
         // stay in uniform registers.
-        constexpr uint32_t IDESC = f16_idesc(kM, BN, true);
+        constexpr uint32_t IDESC = f16_idesc(PAIR ? 2 * kM : kM, BN, true);
+        auto commit = [](uint32_t bar) {
+            if (PAIR) tc_commit_pair(bar);
+            else tc_commit(bar);
+        };
         const bool leader = elect_one();
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
         int st = 0, phase = 0, it = 0;
-        for (int t = blockIdx.x; t < a.tiles && !*abort_flag; t += gridDim.x, ++it) {
+        for (int t = tile_first; t < a.tiles && !*abort_flag; t += tile_step, ++it) {
             const int ab = it & 1;
             if (it >= 2) {
                 mbar_wait_uniform(acc_empty(ab), ((it >> 1) - 1) & 1, abort_addr, &g_linear_status);
@@ -175,22 +203,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint64_t bd = sw128_desc(sa + Cfg::A_BYTES, 64 * kK * 2, 1024);
                 if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < kK / 16; ++kk)
-                        tc_mma(d, ad + kk * (32 >> 4), bd + kk * (2048 >> 4), IDESC, kb > 0 || kk > 0);
-                    tc_commit(empty(st));
+                    for (int kk = 0; kk < kK / 16; ++kk) {
+                        const uint64_t ak = ad + kk * (32 >> 4), bk = bd + kk * (2048 >> 4);
+                        if (PAIR) tc_mma_pair(d, ak, bk, IDESC, kb > 0 || kk > 0);
+                        else tc_mma(d, ak, bk, IDESC, kb > 0 || kk > 0);
+                    }
+                    commit(empty(st));
                 }
                 __syncwarp();
                 if (++st == Cfg::STAGES) st = 0, phase ^= 1;
             }
-            if (leader) tc_commit(acc_full(ab));
+            if (leader) commit(acc_full(ab));
             __syncwarp();
         }
         if (leader) {  // every product has completed before the CTA frees its memory
-            tc_commit(done);
+            commit(done);
             mbar_drain(done, 0);
         }
         __syncwarp();
-    } else {
+    } else if (warp > 1) {
         // ---- epilogue: a warp owns 32 rows and every other 32 columns of the tile.  It works
         // alone: its rows leave through its own buffers and bulk stores, the residual of the
         // next 32 columns is on its way while these are computed.
@@ -202,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
         int it = 0, ob = 0;
-        for (int t = blockIdx.x; t < a.tiles && !*abort_flag; t += gridDim.x, ++it) {
+        for (int t = tile_first; t < a.tiles && !*abort_flag; t += tile_step, ++it) {
             int m, n;
             tile_of(a, t, m, n);
             const int ab = it & 1;
@@ -215,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 named_barrier(1, 32 * kEpiWarps);
             }
-            const int64_t row = static_cast<int64_t>(m) * kM + r;
+            const int64_t row = row_of(m) + r;
             const bool live = row < a.rows;
             uint4 res[4];
             auto load_res = [&](int c0) {
@@ -284,64 +315,90 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    tma_store_2d(&omap, col0, m * kM + quarter * 32, stage_addr + ob * 2048);
+                    tma_store_2d(&omap, col0, row_of(m) + quarter * 32, stage_addr + ob * 2048);
                     bulk_commit();
                 }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty(ab));
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_cluster(cluster_addr(acc_empty(ab), 0));
+                else mbar_arrive(acc_empty(ab));
+            }
         }
         if (lane == 0) bulk_wait<0>();
         __syncwarp();
     }
+    __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    if (PAIR) cluster_sync_all();  // neither CTA leaves while the other one uses its memory
+    else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                     "r"(Cfg::TMEM_COLS)
-                     : "memory");
+        if (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                         "r"(Cfg::TMEM_COLS)
+                         : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                         "r"(Cfg::TMEM_COLS)
+                         : "memory");
     }
 }
 
-// Waves of the grid times the cost of a tile: BN columns take BN / 2 cycles of the tensor cores a K
-// step of 16, and below 128 columns A's 4 KB bound the step by shared memory instead; the constant
-// is what a tile costs beside its products (measured: see choose()).
-inline int64_t cost_of(int64_t m_tiles, int64_t n_tiles, int bn, int64_t ksteps) {
-    const int64_t waves = (m_tiles * n_tiles + device_sm_count() - 1) / device_sm_count();
-    return waves * ((bn > 128 ? bn : 64 + bn / 2) * ksteps + 1500);
+// Time of a whole product in units of a 128 x 1 column of accumulators over 16 of K: waves of the
+// grid times a tile's.  `weight` is a tile's time a K step against 256 for a 128 x 256 tile, which
+// falls more slowly than its columns, because A's part of the shared-memory and L2 traffic stays
+// (measured at 8191 x 4096 x 4096, time a wave: 256 columns 31.1 us, 192 24.7, 128 20.0, 64 15.6;
+// a pair of CTAs, which holds half of W each, 27.2); 1500 is what a tile costs beside its products.
+inline int64_t time_of(int64_t m_tiles, int64_t n_tiles, int units, int weight, int64_t ksteps) {
+    return (m_tiles * n_tiles + units - 1) / units * (weight * ksteps + 1500);
 }
 
-template <int BN, bool GATED>
+template <int BN, bool GATED, bool PAIR = false>
 int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ldo,
            LinArgs a, cudaStream_t s) {
-    using Cfg = LinCfg<BN, GATED>;
+    using Cfg = LinCfg<BN, GATED, PAIR>;
     CUtensorMap xmap, wmap, omap;
     if (int st = make_map(&xmap, x, a.k, a.rows, ldx * 2, kM)) return st;
     if (int st = make_map(&wmap, w, GATED ? 2 * static_cast<int64_t>(a.n) : a.n, a.k, ldw * 2, kK))
         return st;
     if (int st = make_store_map(&omap, out, a.n, a.rows, ldo * 2)) return st;
-    a.m_tiles = (a.rows + kM - 1) / kM;
+    a.m_tiles = PAIR ? (a.rows + 2 * kM - 1) / (2 * kM) : (a.rows + kM - 1) / kM;
     a.n_tiles = (a.n + Cfg::ON - 1) / Cfg::ON;
     int64_t tiles;
     if (!mul_ok(a.m_tiles, a.n_tiles, &tiles) || tiles > INT32_MAX)
         return fail(TMLLM_INVALID_SHAPE, "too many output tiles");
     a.tiles = static_cast<int32_t>(tiles);
-    a.group_m = 16;
+    a.group_m = PAIR ? 8 : 16;
     static std::atomic<uint64_t> opted{0};
     int dev = 0;
     TMLLM_CUDA_TRY(cudaGetDevice(&dev));
     const uint64_t bit = dev < 64 ? (1ull << dev) : 0;
     if (!bit || !(opted.load(std::memory_order_relaxed) & bit)) {
-        TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_linear_kernel<BN, GATED>,
+        TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_linear_kernel<BN, GATED, PAIR>,
                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             Cfg::SMEM));
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
     const int sms = device_sm_count();
-    const unsigned grid = static_cast<unsigned>(tiles < sms ? tiles : sms);
-    prompt_linear_kernel<BN, GATED><<<grid, kThreads, Cfg::SMEM, s>>>(xmap, wmap, omap, a);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg::SMEM;
+    cfg.stream = s;
+    if (PAIR) {
+        const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
+        cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    } else {
+        cfg.gridDim = dim3(static_cast<unsigned>(tiles < sms ? tiles : sms));
+    }
+    TMLLM_CUDA_TRY(cudaLaunchKernelEx(&cfg, prompt_linear_kernel<BN, GATED, PAIR>, xmap, wmap, omap, a));
     TMLLM_LAUNCH_TRY();
     return TMLLM_OK;
 }
@@ -402,21 +459,34 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     a.n = n;
     a.act = activation;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const int64_t mt = (rows + kM - 1) / kM, ksteps = (k + 15) / 16;
+    // the fastest tile by that model: few or ragged tiles take narrow ones, large products a pair
+    // of CTAs (8191 x 4096 x 4096: 190 us against 218 alone, back to back under the power limit)
+    const int64_t mt = (rows + kM - 1) / kM, mp = (rows + 2 * kM - 1) / (2 * kM);
+    const int64_t ksteps = (k + 15) / 16;
+    const int sms = device_sm_count();
     auto tiles = [&](int on) { return (static_cast<int64_t>(n) + on - 1) / on; };
     if (activation == ACT_SWIGLU) {
-        const bool wide_tile = cost_of(mt, tiles(128), 256, ksteps) <= cost_of(mt, tiles(64), 128, ksteps);
-        return wide_tile ? launch<256, true>(x, ldx, w, ldw, out, ldo, a, s)
-                         : launch<128, true>(x, ldx, w, ldw, out, ldo, a, s);
+        const int64_t t256 = time_of(mt, tiles(128), sms, 256, ksteps);
+        const int64_t t128 = time_of(mt, tiles(64), sms, 170, ksteps);
+        const int64_t pair = time_of(mp, tiles(128), sms / 2, 224, ksteps);
+        if (pair < t256 && pair < t128)
+            return launch<256, true, true>(x, ldx, w, ldw, out, ldo, a, s);
+        return t256 <= t128 ? launch<256, true>(x, ldx, w, ldw, out, ldo, a, s)
+                            : launch<128, true>(x, ldx, w, ldw, out, ldo, a, s);
     }
-    int best = 256;
-    for (int bn : {192, 128, 64})
-        if (cost_of(mt, tiles(bn), bn, ksteps) < cost_of(mt, tiles(best), best, ksteps)) best = bn;
+    const int64_t times[5] = {
+        time_of(mt, tiles(64), sms, 130, ksteps), time_of(mt, tiles(128), sms, 170, ksteps),
+        time_of(mt, tiles(192), sms, 210, ksteps), time_of(mt, tiles(256), sms, 256, ksteps),
+        time_of(mp, tiles(256), sms / 2, 224, ksteps)};
+    int best = 0;
+    for (int i = 1; i < 5; ++i)
+        if (times[i] < times[best]) best = i;
     switch (best) {
-        case 64: return launch<64, false>(x, ldx, w, ldw, out, ldo, a, s);
-        case 128: return launch<128, false>(x, ldx, w, ldw, out, ldo, a, s);
-        case 192: return launch<192, false>(x, ldx, w, ldw, out, ldo, a, s);
-        default: return launch<256, false>(x, ldx, w, ldw, out, ldo, a, s);
+        case 0: return launch<64, false>(x, ldx, w, ldw, out, ldo, a, s);
+        case 1: return launch<128, false>(x, ldx, w, ldw, out, ldo, a, s);
+        case 2: return launch<192, false>(x, ldx, w, ldw, out, ldo, a, s);
+        case 3: return launch<256, false>(x, ldx, w, ldw, out, ldo, a, s);
+        default: return launch<256, false, true>(x, ldx, w, ldw, out, ldo, a, s);
     }
 }
 

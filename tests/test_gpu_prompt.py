@@ -470,6 +470,14 @@ def test_prompt_linear_strides_and_place(cuda):
     linear_case(cuda, 4097, 512, 520, "swiglu", bias=True, seed=5)
 
 
+@pytest.mark.parametrize("rows,k,n", [(2304, 264, 2048), (2049, 72, 2040), (16640, 64, 256)])
+def test_prompt_linear_pairs_of_ctas(cuda, rows, k, n):
+    """Sizes whose tiles fit one wave of CTA pairs, with a last pair that is not full."""
+    linear_case(cuda, rows, k, n, "gelu", bias=True, seed=1)
+    linear_case(cuda, rows, k, n, residual=True, inplace=True, seed=2)
+    linear_case(cuda, rows, k, n // 2 + 8 - n // 2 % 8, "swiglu", bias=True, residual=True, seed=3)
+
+
 def test_prompt_linear_non_finite_rows_stay_apart(cuda):
     """NaN in one row of x, or past k in its buffer, reaches that row alone."""
     x = torch.ones(200, 128, dtype=torch.float16, device=cuda)
