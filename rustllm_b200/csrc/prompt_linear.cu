@@ -65,7 +65,7 @@ struct LinCfg {
     static constexpr int OFF_OUT = STAGES * STAGE;
     static constexpr int OFF_BIAS = OFF_OUT + kEpiWarps * 2 * 2048;
     static constexpr int OFF_BAR = OFF_BIAS + 2 * BN * 2;  // bias as F16
-    static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment
+    static constexpr int SMEM = OFF_BAR + 512 + 1024;  // + alignment
     static constexpr int ACC = BN <= 64 ? 64 : BN <= 128 ? 128 : 256;  // columns apart
     static constexpr int TMEM_COLS = 2 * ACC;                          // two accumulators
     static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
@@ -86,7 +86,8 @@ template <int BN, bool GATED, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_linear_kernel(const __grid_constant__ CUtensorMap xmap,
                          const __grid_constant__ CUtensorMap wmap,
-                         const __grid_constant__ CUtensorMap omap, const LinArgs a) {
+                         const __grid_constant__ CUtensorMap omap,
+                         const __grid_constant__ CUtensorMap rmap, const LinArgs a) {
     using Cfg = LinCfg<BN, GATED, PAIR>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -99,7 +100,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto acc_full = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + i); };
     auto acc_empty = [&](int i) { return bars + 8u * (2 * Cfg::STAGES + 2 + i); };
     const uint32_t done = bars + 8u * (2 * Cfg::STAGES + 4);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 8 * (2 * Cfg::STAGES + 5));
+    auto res_full = [&](int w, int b) { return bars + 8u * (2 * Cfg::STAGES + 5 + 2 * w + b); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(
+        smem + Cfg::OFF_BAR + 8 * (2 * Cfg::STAGES + 5 + 2 * kEpiWarps));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     if (tid == 0) {
@@ -112,6 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(acc_empty(i), kEpiWarps * (PAIR ? 2 : 1));
         }
         mbar_init(done, 1);
+        for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(res_full(i >> 1, i & 1), 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -223,16 +227,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     } else if (warp > 1) {
         // ---- epilogue: a warp owns 32 rows and every other 32 columns of the tile.  It works
-        // alone: its rows leave through its own buffers and bulk stores, the residual of the
-        // next 32 columns is on its way while these are computed.
+        // alone: its rows leave through its own two buffers and bulk stores; the residual
+        // arrives the same way in the buffer it leaves by, 32 columns ahead.
         const int quarter = warp & 3, part = (warp - 2) >> 2;
-        const int r = quarter * 32 + lane;  // this thread's row of the tile (its lane)
         __half* bias_s = reinterpret_cast<__half*>(smem + Cfg::OFF_BIAS);
         unsigned char* stage = smem + Cfg::OFF_OUT + (warp - 2) * 4096;
         const uint32_t stage_addr = smem_u32(stage);
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
         int it = 0, ob = 0;
+        uint32_t phases[2] = {0u, 0u};
         for (int t = tile_first; t < a.tiles && !*abort_flag; t += tile_step, ++it) {
             int m, n;
             tile_of(a, t, m, n);
@@ -246,19 +250,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 named_barrier(1, 32 * kEpiWarps);
             }
-            const int64_t row = row_of(m) + r;
-            const bool live = row < a.rows;
-            uint4 res[4];
-            auto load_res = [&](int c0) {
+            // columns c0 .. of the tile into buffer b, once its last store has been read
+            auto load_res = [&](int c0, int b) {
                 const int col = n * Cfg::ON + c0;
-                const __half* p = a.residual + row * a.ld_res + col;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    res[j] = live && c0 < Cfg::ON && col + 8 * j < a.n
-                                 ? *reinterpret_cast<const uint4*>(p + 8 * j)
-                                 : make_uint4(0u, 0u, 0u, 0u);
+                if (!a.residual || c0 >= Cfg::ON || col >= a.n || lane != 0) return;
+                bulk_wait_read<0>();
+                mbar_arrive_tx(res_full(warp - 2, b), 2048);
+                tma_load_2d(stage_addr + b * 2048, &rmap, col, row_of(m) + quarter * 32,
+                            res_full(warp - 2, b));
             };
-            if (a.residual) load_res(part * 32);
+            load_res(part * 32, ob);
             mbar_wait_uniform(acc_full(ab), (it >> 1) & 1, abort_addr, &g_linear_status);
             tc_fence_after();
             const uint32_t acc = tmem + ab * Cfg::ACC + lane_base;
@@ -291,20 +292,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) y[i] = relu(y[i]);
                 }
+                unsigned char* srow = stage + ob * 2048 + lane * 64;  // 64-byte swizzle
                 if (a.residual) {
+                    load_res(c0 + 64, ob ^ 1);
+                    mbar_wait_uniform(res_full(warp - 2, ob), phases[ob], abort_addr,
+                                      &g_linear_status);
+                    phases[ob] ^= 1;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float f[8];
-                        Chunk<__half>::unpack(res[j], f);
+                        Chunk<__half>::unpack(*reinterpret_cast<const uint4*>(
+                                                  srow + ((j ^ (lane >> 1 & 3)) << 4)),
+                                              f);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) y[8 * j + e] += f[e];
                     }
-                    load_res(c0 + 64);
+                } else {
+                    // the buffer of two stores ago has been read
+                    if (lane == 0) bulk_wait_read<1>();
+                    __syncwarp();
                 }
-                // the buffer of two stores ago has been read
-                if (lane == 0) bulk_wait_read<1>();
-                __syncwarp();
-                unsigned char* srow = stage + ob * 2048 + lane * 64;  // 64-byte swizzle
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     *reinterpret_cast<uint4*>(srow + ((j ^ (lane >> 1 & 3)) << 4)) =
@@ -364,6 +371,9 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, in
     if (int st = make_map(&wmap, w, GATED ? 2 * static_cast<int64_t>(a.n) : a.n, a.k, ldw * 2, kK))
         return st;
     if (int st = make_store_map(&omap, out, a.n, a.rows, ldo * 2)) return st;
+    CUtensorMap rmap = omap;
+    if (a.residual)
+        if (int st = make_store_map(&rmap, a.residual, a.n, a.rows, a.ld_res * 2)) return st;
     a.m_tiles = PAIR ? (a.rows + 2 * kM - 1) / (2 * kM) : (a.rows + kM - 1) / kM;
     a.n_tiles = (a.n + Cfg::ON - 1) / Cfg::ON;
     int64_t tiles;
@@ -398,7 +408,8 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, in
     } else {
         cfg.gridDim = dim3(static_cast<unsigned>(tiles < sms ? tiles : sms));
     }
-    TMLLM_CUDA_TRY(cudaLaunchKernelEx(&cfg, prompt_linear_kernel<BN, GATED, PAIR>, xmap, wmap, omap, a));
+    TMLLM_CUDA_TRY(cudaLaunchKernelEx(&cfg, prompt_linear_kernel<BN, GATED, PAIR>, xmap, wmap, omap,
+                                      rmap, a));
     TMLLM_LAUNCH_TRY();
     return TMLLM_OK;
 }

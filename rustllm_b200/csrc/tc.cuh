@@ -19,7 +19,7 @@ namespace tmllm {
 int make_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t row_bytes,
              int box_rows, bool f32 = false);
 
-// For stores from buffers of 32 rows x 32 F16 columns in the 64-byte swizzle (chunk c of row r at
+// For stores from (and loads into) buffers of 32 rows x 32 F16 columns in the 64-byte swizzle (chunk c of row r at
 // chunk c ^ (r / 2 % 4)).
 int make_store_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows,
                    int64_t row_bytes);
