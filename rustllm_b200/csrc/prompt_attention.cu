@@ -320,8 +320,8 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 // its rows are read to registers (and the next step's S is computed over it), exponentiated, and P
 // is written to columns of its own as F16, from where it is the A operand of O += P V, so only V
 // crosses shared memory for the second product.
-//   tensor memory, KS keys a step: S_i at [KS i, + KS), P_i at [2 KS + KS / 2 i, + KS / 2), O_i at
-//   [512 - DP (2 - i), + DP)
+//   tensor memory, KS keys a step, PB buffers of P: S_i at [KS i, + KS), P_i[b] at [2 KS +
+//   KS / 2 (PB i + b), + KS / 2), O_i at [512 - DP (2 - i), + DP)
 //
 // Masked places never reach a result: scores that a row does not see are replaced by -inf before
 // the maximum, and since 0 * inf is not 0, the non-finite entries of every V tile that some row
@@ -347,13 +347,14 @@ struct AttCfg {
     static constexpr int OFF_BAR = OFF_OUT + 8 * 2048;
     static constexpr int KS = DP == 64 ? 128 : 64;  // keys of a step
     static constexpr int SPT = 128 / KS;            // steps of a key tile
-    static_assert(3 * KS + 2 * DP <= 512, "tensor memory");
+    static constexpr int PB = DP == 64 ? 1 : 2;     // buffers of P
+    static_assert(2 * KS + PB * KS + 2 * DP <= 512, "tensor memory");
     static constexpr int SMEM = OFF_BAR + 512 + 1024;  // + alignment
     static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 };
 
 // Barriers: QF/QE Q tile full / empty, KF/KE ring full / empty; of each item: S scores ready, F
-// scores read, P probabilities written, O product done, E accumulator read, VR a V tile to scrub
+// scores read, P probabilities written, O product done (these two of each buffer of P), E accumulator read, VR a V tile to scrub
 // has landed, SB it is scrubbed; DONE all products.  Both MMA warps give back every K and V tile,
 // whether their item uses it or not, so neither falls more than a phase behind the ring, and a
 // softmax group follows its MMA warp step by step.
@@ -362,7 +363,7 @@ struct AttBar {
     using Cfg = AttCfg<DP>;
     static constexpr int QF = 0, QE = QF + 2 * Cfg::QBUF, KF = QE + 2 * Cfg::QBUF,
                          KE = KF + Cfg::STAGES, S = KE + Cfg::STAGES, F = S + 2, P = F + 2,
-                         O = P + 2, E = O + 2, VR = E + 2, SB = VR + 2, DONE = SB + 2,
+                         O = P + 2 * Cfg::PB, E = O + 2 * Cfg::PB, VR = E + 2, SB = VR + 2, DONE = SB + 2,
                          COUNT = DONE + 1;
     static_assert(COUNT * 8 + 64 <= 512, "barrier area");
 };
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      const __grid_constant__ CUtensorMap vmap, const PromptArgs a, int tile0) {
     using Cfg = AttCfg<DP>;
     using B = AttBar<DP>;
-    constexpr int KS = Cfg::KS, SPT = Cfg::SPT;
+    constexpr int KS = Cfg::KS, SPT = Cfg::SPT, PB = Cfg::PB;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
@@ -586,7 +587,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     auto tmem_s = [&](int i) { return tmem + static_cast<uint32_t>(KS * i); };
-    auto tmem_p = [&](int i) { return tmem + static_cast<uint32_t>(2 * KS + KS / 2 * i); };
+    auto tmem_p = [&](int i, int b) {
+        return tmem + static_cast<uint32_t>(2 * KS + KS / 2 * (PB * i + b));
+    };
     auto tmem_o = [&](int i) { return tmem + static_cast<uint32_t>(512 - DP * (2 - i)); };
     auto wait = [&](int b, uint32_t parity) {
         return mbar_wait_bounded(bar(b), parity & 1u, abort_flag, &g_attention_status);
@@ -601,7 +604,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int w = warp >> 2, r = tid & 127;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem_s(w) + lane_base, to = tmem_o(w) + lane_base;
-        const uint32_t tp = tmem_p(w) + lane_base;
         unsigned char* stage = smem + Cfg::OFF_OUT + warp * 2048;
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
         int step = 0, ring0 = 0, events = 0;
@@ -656,6 +658,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int n = lo; n <= hi; ++n) {
                 const bool ragged = u.ragged(n / SPT);
                 if (ragged && (n % SPT == 0 || n == lo)) scrub(n / SPT);
+                const int pb = step % PB;  // this step's buffer of P
+                const uint32_t tp = tmem_p(w, pb) + lane_base;
                 await(B::S + w, step);
                 tc_fence_after();
                 float v[KS];
@@ -687,71 +691,60 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                     }
                 }
-                auto row_max = [&]() {
-                    float mx[4] = {v[0], v[1], v[2], v[3]};
+                float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int i = 4; i < KS - 4; i += 8)
+                for (int i = 4; i < KS - 4; i += 8)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], v[i + e], v[i + 4 + e]);
-                    return fmaxf(max3(mx[0], mx[1], fmaxf(v[KS - 4], v[KS - 3])),
-                                 max3(mx[2], mx[3], fmaxf(v[KS - 2], v[KS - 1]))) *
-                           a.scale_log2;
-                };
-                // P is taken relative to the running maximum m of the steps before, which is
-                // known at once, and this step's own maximum is found meanwhile.  Only when it
-                // exceeds m by more than 2^8 does m follow (P is computed again, O and l are
-                // rescaled); else P stays below 2^8 and 1 / l makes up for it.
-                // A row's first visible step (m = -inf: its l and O are zero) takes its maximum.
-                const bool begin = n == lo;
-                const bool fresh = m == -INFINITY;
-                if (__any_sync(FULL, fresh)) {
-                    const float mt = row_max();
-                    if (fresh) m = mt;
-                }
+                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], v[i + e], v[i + 4 + e]);
+                const float mt = fmaxf(max3(mx[0], mx[1], fmaxf(v[KS - 4], v[KS - 3])),
+                                       max3(mx[2], mx[3], fmaxf(v[KS - 2], v[KS - 1]))) *
+                                 a.scale_log2;
+                // The running maximum m follows only when a row's grew by more than 2^8 (then O and
+                // l are rescaled); else P stays below 2^8 and 1 / l makes up for it.  A row's first
+                // visible step (m = -inf: its l and O are zero) takes its maximum.
                 float alpha = 1.f;
-                bool grown = false;  // of some row of the warp
-                float2 l2[2];
-                for (;;) {
-                    // -inf (nothing visible yet): exp2(-inf - 0) = 0
-                    const float sub = m == -INFINITY ? 0.f : -m;
-                    const float2 sub2 = make_float2(sub, sub);
-                    l2[0] = l2[1] = make_float2(0.f, 0.f);
-#pragma unroll
-                    for (int c = 0; c < KS / 32; ++c) {
-                        uint32_t pk[16];
-                        // 32 columns no row of the warp sees: zeros without exponentials
-                        if (!(dark >> c & 1u)) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const int i = c * 32 + 2 * e;
-                                const float2 x = __ffma2_rn(make_float2(v[i], v[i + 1]), sc2, sub2);
-                                const float2 p = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-                                l2[e & 1] = __fadd2_rn(l2[e & 1], p);
-                                pk[e] = pack_half2(p.x, p.y);
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) pk[e] = 0u;
-                        }
-                        if (c == 0 && !begin) {  // the product before has read P
-                            await(B::O + w, step - 1);
-                            tc_fence_after();
-                        }
-                        tmem_st16_bits(tp + 16 * c, pk);
-                    }
-                    if (begin || dark == (1u << (KS / 32)) - 1u) break;
-                    const float mt = row_max();
-                    const bool grow = mt > m + 8.f;
-                    if (!__any_sync(FULL, grow)) break;
-                    grown = true;
-                    if (grow) {
+                const bool fresh = m == -INFINITY, grow = mt > m + 8.f;
+                if (grow) {
+                    if (!fresh) {
                         alpha = exp2_approx(m - mt);
                         l *= alpha;
-                        m = mt;
                     }
+                    m = mt;
+                }
+                const bool rescale = __any_sync(FULL, grow && !fresh);
+                // -inf (nothing visible yet): exp2(-inf - 0) = 0
+                const float sub = m == -INFINITY ? 0.f : -m;
+                const float2 sub2 = make_float2(sub, sub);
+                float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < KS / 32; ++c) {
+                    uint32_t pk[16];
+                    // 32 columns no row of the warp sees: zeros without exponentials
+                    if (!(dark >> c & 1u)) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int i = c * 32 + 2 * e;
+                            const float2 x = __ffma2_rn(make_float2(v[i], v[i + 1]), sc2, sub2);
+                            const float2 p = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                            l2[e & 1] = __fadd2_rn(l2[e & 1], p);
+                            pk[e] = pack_half2(p.x, p.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) pk[e] = 0u;
+                    }
+                    if (c == 0 && step >= PB) {  // the buffer's last product has read it
+                        await(B::O + PB * w + pb, step / PB - 1);
+                        tc_fence_after();
+                    }
+                    tmem_st16_bits(tp + 16 * c, pk);
                 }
                 l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
-                if (grown) {  // O holds the products before this step
+                if (rescale) {  // O is to hold the products before this step
+                    if (PB == 2) {
+                        await(B::O + PB * w + (pb ^ 1), (step - 1) / PB);
+                        tc_fence_after();
+                    }
 #pragma unroll 1
                     for (int c = 0; c < DP / 32; ++c) {
                         float o[32];
@@ -763,13 +756,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(bar(B::P + w));
+                mbar_arrive(bar(B::P + PB * w + pb));
                 ++step;
             }
             ring0 += 2 * (u.jhi - u.jlo + 1);
             if (!on) continue;
             // ---- epilogue
-            await(B::O + w, step - 1);
+            await(B::O + PB * w + (step - 1) % PB, (step - 1) / PB);
             tc_fence_after();
             const bool odd = *odd_flag != 0;
             const float inv = l == 0.f ? 0.f : 1.f / l;  // every score -inf: zeros
@@ -939,21 +932,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const bool mine = n >= lo && n <= hi;
                 if (sub == 0) await_full(x);
                 if (mine) {
-                    await(B::P + i, prods);
+                    await(B::P + PB * i + prods % PB, prods / PB);
                     // the accumulator still holds this item's previous unit
                     if (n == lo && units > 0) await(B::E + i, units - 1);
                     tc_fence_after();
                 }
                 const uint32_t va = sbase + Cfg::OFF_KV + stage_of(x) * Cfg::TILE + sub * KS * 128;
                 const uint64_t vd = sw128_desc(va, Cfg::BLK, 1024);
-                const uint32_t d = tmem_o(i), p = tmem_p(i);
+                const uint32_t d = tmem_o(i), p = tmem_p(i, prods % PB);
                 if (leader) {
                     if (mine) {
 #pragma unroll
                         for (int kk = 0; kk < KS / 16; ++kk)
                             tc_mma_ts(d, p + 8u * kk, vd + kk * (2048 >> 4), IDESC_PV,
                                       n > lo || kk > 0);
-                        tc_commit(bar(B::O + i));
+                        tc_commit(bar(B::O + PB * i + prods % PB));
                     }
                     if (sub == SPT - 1) tc_commit(bar(B::KE + stage_of(x)));
                 }
