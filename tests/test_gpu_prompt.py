@@ -375,6 +375,13 @@ def test_prompt_attention_long(cuda):
     attention_case(cuda, [1500], 2, 1, 128, seed=2)
 
 
+def test_prompt_attention_many_rows(cuda):
+    """More packed rows than one launch schedules (131,072), tiles shared by two or three
+    sequences, and one sequence across the border."""
+    attention_case(cuda, [100] * 1305 + [900] + [77] * 60, 1, 1, 32, seed=1, pad=40)
+    attention_case(cuda, [60] * 2190, 2, 1, 72, seed=2)
+
+
 def test_prompt_attention_forms(cuda):
     attention_case(cuda, [70, 200], 4, 2, 64, out_dtype=torch.float32, seed=1)
     attention_case(cuda, [70, 200], 4, 2, 64, scale=0.7, seed=2)     # sharp rows
