@@ -315,6 +315,7 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 //   warps 0-3, 4-7  softmax of item 0 / 1, one thread a query row
 //   warp 8          TMA producer: Q tiles, then K and V tiles through a ring
 //   warps 9, 10     MMA issuers of item 0 / 1
+//   warp 11         scrub (below)
 // K and V arrive in tiles of 128 keys and are used in steps of 128 keys, or of 64 above head size
 // 64, where the accumulators leave less tensor memory.  S = Q K^T of a step sits in tensor memory;
 // its rows are read to registers (and the next step's S is computed over it), exponentiated, and P
@@ -329,7 +330,7 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 // afterwards to the rows that see them ("scrubbed" tiles: the diagonal, the tile where the
 // sequence starts, all tiles of an item whose rows belong to several sequences).
 constexpr int kTile = 128;
-constexpr int kTcThreads = 384;  // warp 11 completes a warpgroup and idles
+constexpr int kTcThreads = 384;
 constexpr int kWindow = 1024;    // row tiles a launch schedules (131,072 packed rows)
 
 template <int DP>
@@ -353,17 +354,17 @@ struct AttCfg {
     static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 };
 
-// Barriers: QF/QE Q tile full / empty, KF/KE ring full / empty; of each item: S scores ready, F
-// scores read, P probabilities written, O product done (these two of each buffer of P), E accumulator read, VR a V tile to scrub
-// has landed, SB it is scrubbed; DONE all products.  Both MMA warps give back every K and V tile,
-// whether their item uses it or not, so neither falls more than a phase behind the ring, and a
-// softmax group follows its MMA warp step by step.
+// Barriers: QF/QE Q tile full / empty, KF/KE ring full / empty, SB V tile of a ring stage ready for
+// the product; of each item: S scores ready, F scores read, P probabilities written, O product done
+// (these two of each buffer of P), E accumulator read; DONE all products.  Both MMA warps give back
+// every K and V tile, whether their item uses it or not, so no role falls more than a phase behind
+// the ring.
 template <int DP>
 struct AttBar {
     using Cfg = AttCfg<DP>;
     static constexpr int QF = 0, QE = QF + 2 * Cfg::QBUF, KF = QE + 2 * Cfg::QBUF,
                          KE = KF + Cfg::STAGES, S = KE + Cfg::STAGES, F = S + 2, P = F + 2,
-                         O = P + 2 * Cfg::PB, E = O + 2 * Cfg::PB, VR = E + 2, SB = VR + 2, DONE = SB + 2,
+                         O = P + 2 * Cfg::PB, E = O + 2 * Cfg::PB, SB = E + 2, DONE = SB + Cfg::STAGES,
                          COUNT = DONE + 1;
     static_assert(COUNT * 8 + 64 <= 512, "barrier area");
 };
@@ -523,8 +524,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     if (tid == 0) {
         for (int i = 0; i < B::COUNT; ++i) {
-            const bool group = (i >= B::F && i < B::O) || (i >= B::E && i < B::VR) ||
-                               (i >= B::SB && i < B::DONE);
+            const bool group = (i >= B::F && i < B::O) || (i >= B::E && i < B::SB);
             const bool both = i == B::DONE || (i >= B::KE && i < B::KE + Cfg::STAGES);
             mbar_init(bar(i), group ? 128u : both ? 2u : 1u);
         }
@@ -631,39 +631,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t ts = tmem_s(w) + lane_base, to = tmem_o(w) + lane_base;
         unsigned char* stage = smem + Cfg::OFF_OUT + warp * 2048;
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
-        int step = 0, ring0 = 0, events = 0;
+        int step = 0;
         auto await = [&](int b, int phase) {
             mbar_wait_uniform(bar(b), phase & 1, abort_addr, &g_attention_status);
-        };
-        // Non-finite entries of the V tile of key tile j become zeros, and the flag says that some
-        // were found.  Each group does it for its own item: the other one may be on the same
-        // tile, writing the same zeros (the flag comes first, so who sees a zero sees the flag).
-        auto scrub = [&](int j) {
-            const int st = (ring0 + 2 * (j - u.jlo) + 1) % Cfg::STAGES;
-            await(B::VR + w, events++);
-            unsigned char* v = smem + Cfg::OFF_KV + st * Cfg::TILE + r * 16;
-            __half2 probe = __floats2half2_rn(0.f, 0.f);
-            const __half2 zero = probe;
-#pragma unroll
-            for (int c = 0; c < DP / 8; ++c) {
-                const uint4 x = *reinterpret_cast<const uint4*>(v + 2048 * c);
-                const __half2* h = reinterpret_cast<const __half2*>(&x);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) probe = __hfma2(h[e], zero, probe);  // 0 or NaN
-            }
-            if (!(__low2float(probe) == 0.f && __high2float(probe) == 0.f)) {
-                *odd_flag = 1;
-                __threadfence_block();
-                for (int c = 0; c < DP / 8; ++c) {
-                    for (int e = 0; e < 8; ++e) {
-                        volatile uint16_t* b = reinterpret_cast<volatile uint16_t*>(v + 2048 * c) + e;
-                        if (odd_half(*b)) *b = 0;
-                    }
-                }
-                fence_async_smem();
-            }
-            __syncwarp();
-            mbar_arrive(bar(B::SB + w));
         };
         const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
         while (sched.template next<Cfg::KS>(a, u) && !*abort_flag) {
@@ -681,7 +651,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             float m = -INFINITY, l = 0.f;
             for (int n = lo; n <= hi; ++n) {
                 const bool ragged = u.ragged(n / SPT);
-                if (ragged && (n % SPT == 0 || n == lo)) scrub(n / SPT);
                 const int pb = step % PB;  // this step's buffer of P
                 const uint32_t tp = tmem_p(w, pb) + lane_base;
                 await(B::S + w, step);
@@ -785,12 +754,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 mbar_arrive(bar(B::P + PB * w + pb));
                 ++step;
             }
-            ring0 += 2 * (u.jhi - u.jlo + 1);
             if (!on) continue;
             // ---- epilogue
             await(B::O + PB * w + (step - 1) % PB, (step - 1) / PB);
             tc_fence_after();
-            __threadfence_block();
             const bool odd = *odd_flag != 0;
             const float inv = l == 0.f ? 0.f : 1.f / l;  // every score -inf: zeros
             const int64_t orow = (live ? row : 0) * a.out_stride +
@@ -915,7 +882,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const bool leader = elect_one();
             const int ksteps = (a.head_dim + 15) / 16;
             const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
-            int ring0 = 0, units = 0, scores = 0, prods = 0, events = 0;
+            int ring0 = 0, units = 0, scores = 0, prods = 0;
             auto await = [&](int b, int phase) {
                 mbar_wait_uniform(bar(b), phase & 1, abort_addr, &g_attention_status);
             };
@@ -957,7 +924,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int sub = n % SPT;
                 const int x = ring0 + 2 * (n / SPT - u.jlo) + 1;
                 const bool mine = n >= lo && n <= hi;
-                if (sub == 0) await_full(x);
+                if (sub == 0) await(B::SB + stage_of(x), x / Cfg::STAGES);
                 if (mine) {
                     await(B::P + PB * i + prods % PB, prods / PB);
                     // the accumulator still holds this item's previous unit
@@ -980,29 +947,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 if (mine) ++prods;
             };
-            // step n's is the item's first use of a V tile that is scrubbed before
-            auto scrubs = [&](int n) {
-                return n >= lo && n <= hi && (n % SPT == 0 || n == lo) && u.ragged(n / SPT);
-            };
-            auto v_ready = [&](int n) {
-                if (!scrubs(n)) return;
-                await_full(ring0 + 2 * (n / SPT - u.jlo) + 1);
-                if (leader) mbar_arrive(bar(B::VR + i));
-                __syncwarp();
-            };
             while (sched.template next<Cfg::KS>(a, u) && !*abort_flag) {
                 u.make_uniform();
                 lo = i ? u.lo[1] : u.lo[0];
                 hi = i ? u.hi[1] : u.hi[0];
                 const int n0 = u.jlo * SPT, n1 = u.jhi * SPT + SPT - 1;
                 qk(n0);
-                v_ready(n0);
                 for (int n = n0; n <= n1; ++n) {
-                    if (scrubs(n)) await(B::SB + i, events++);
-                    if (n < n1) {
-                        qk(n + 1);
-                        v_ready(n + 1);
-                    }
+                    if (n < n1) qk(n + 1);
                     pv(n);
                 }
                 ring0 += 2 * (u.jhi - u.jlo + 1);
@@ -1012,6 +964,48 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (leader) {  // every product is done before the CTA frees its memory
                 tc_commit(bar(B::DONE));
                 mbar_drain(bar(B::DONE), 0);
+            }
+        } else if (warp == 11) {
+            // ---- scrub: a V tile that some row of the unit does not see whole loses its
+            // non-finite entries (and the flag says that some were found) before the products
+            // read it, while the softmax groups are at its scores
+            const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
+            int x = 1;  // ring index of the V tile
+            while (sched.template next<Cfg::KS>(a, u) && !*abort_flag) {
+                for (int j = u.jlo; j <= u.jhi; ++j, x += 2) {
+                    const int st = x % Cfg::STAGES;
+                    mbar_wait_uniform(bar(B::KF + st), (x / Cfg::STAGES) & 1, abort_addr,
+                                      &g_attention_status);
+                    if (u.ragged(j)) {
+                        unsigned char* v = smem + Cfg::OFF_KV + st * Cfg::TILE + lane * 16;
+                        __half2 probe[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) probe[e] = __floats2half2_rn(0.f, 0.f);
+                        const __half2 zero = probe[0];
+#pragma unroll 8
+                        for (int c = 0; c < Cfg::TILE / 512; ++c) {
+                            const uint4 y = *reinterpret_cast<const uint4*>(v + 512 * c);
+                            const __half2* h = reinterpret_cast<const __half2*>(&y);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                probe[e] = __hfma2(h[e], zero, probe[e]);  // 0 or NaN
+                        }
+                        const __half2 sum = __hadd2(__hadd2(probe[0], probe[1]),
+                                                    __hadd2(probe[2], probe[3]));
+                        if (!(__low2float(sum) == 0.f && __high2float(sum) == 0.f)) {
+                            *odd_flag = 1;
+                            for (int c = 0; c < Cfg::TILE / 512; ++c) {
+                                uint16_t* b = reinterpret_cast<uint16_t*>(v + 512 * c);
+                                for (int e = 0; e < 8; ++e)
+                                    if (odd_half(b[e])) b[e] = 0;
+                            }
+                            fence_async_smem();
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(B::SB + st));
+                    __syncwarp();
+                }
             }
         }
     }
