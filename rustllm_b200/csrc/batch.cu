@@ -10,7 +10,7 @@ namespace {
 constexpr int kTabThreads = 256;
 constexpr int kTabItems = 4;                          // requests per thread and round
 constexpr int kTabTile = kTabThreads * kTabItems;     // requests scanned per round
-constexpr int kTabRows = 1024;                        // rows per CTA before the grid grows
+constexpr int kTabRows = 512;                         // rows per CTA before the grid grows
 
 struct TableArgs {
     int32_t* block_table;
