@@ -412,7 +412,7 @@ int tmllm_prefill_status(int32_t* status);
  * rows of the batch, requests refused, rows beyond the capacity}.
  * A request is refused - its rows get position and slot -1 and it takes no block - when its
  * cached length is negative, its tokens pass max_blocks_per_seq * block_size, or it needs
- * blocks and the needs of all requests up to it pass num_free.  Prefix sums are 64-bit and
+ * blocks and *free_start is negative or the needs of all requests up to it pass num_free.  Prefix sums are 64-bit and
  * saturate in the int32 outputs.  The result depends on the arguments alone: calling again
  * with the same arguments gives the same tables. */
 int tmllm_batch_tables(const tmllm_paged_kv* kv, const int32_t* new_lens,

@@ -120,7 +120,8 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const TableAr
         for (int i = 0; i < kTabItems; ++i) {
             const int t = tid * kTabItems + i, s = base + t;
             const bool placed =
-                fits[i] && (need[i] == 0 || start + pb + need[i] <= a.num_free);
+                fits[i] &&
+                (need[i] == 0 || (start >= 0 && start + pb + need[i] <= a.num_free));
             row0[t] = pr;
             from[t] = start + pb;
             cached[t] = placed ? len[i] : -1;

@@ -93,7 +93,11 @@ def _stride(t: torch.Tensor, heads: int, d: int, what: str) -> int:
         raise _lib.ModelFormat(f"{what} must be [rows, {heads}, {d}], got {list(shape)}")
     if stride[2] != 1 and d > 1 or stride[1] != d and heads > 1:
         raise _lib.NonContiguousTensor(f"{what} heads must be packed rows of {d} elements")
-    return stride[0] if shape[0] > 1 else 0
+    if shape[0] <= 1:
+        return 0
+    if stride[0] < heads * d:  # rows over one another (an expanded tensor)
+        raise _lib.NonContiguousTensor(f"{what} rows overlap: stride {stride[0]}")
+    return stride[0]
 
 
 def batch_tables(kv: PagedKV, new_lens: torch.Tensor, rows: int, *,

@@ -121,6 +121,12 @@ def test_batch_tables_refusals_on_the_device(cuda):
     check_tables(cuda, table, lens, [0] * 6, bs, 16, 0, [1])
     check_tables(cuda, table, lens, new, bs, 16, 24, None)  # -1 and 99 are no blocks: slot -1
     check_tables(cuda, table, lens, new, bs, 16, 7, [10, 11, 12])  # fewer rows than tokens
+    check_tables(cuda, table, lens, new, bs, 16, 24, [10, 11, 12], 2)
+    # a negative start of the free list (only requests that need no block are placed)
+    got = run_tables(cuda, table, lens, new, bs, 16, 24, [10, 11, 12], -1)
+    assert got[0] == table and got[5] == [-1, 20, 4, 0]
+    assert got[2][1:3] == [2, 3] and got[2][17:20] == [5, 6, 7]
+    assert set(got[2][:1] + got[2][3:17] + got[2][20:]) == {-1}
     # a free list holding an id outside the pool: kept in the table, no slot
     check_tables(cuda, table, lens, new, bs, 16, 24, [77, 10, 11])
 
@@ -501,6 +507,49 @@ def test_prompt_linear_overflow_is_inf(cuda):
     x = torch.full((3, 64), 300.0, dtype=torch.float16, device=cuda)
     y = rb.prompt_linear(x, torch.full((64, 8), 30.0, dtype=torch.float16, device=cuda))
     assert bool((y == math.inf).all())
+
+
+# ---- refusals of the Python layer -------------------------------------------------------
+def test_python_refusals(cuda):
+    h = dict(dtype=torch.float16, device=cuda)
+    q, k, w = torch.zeros(4, 4, 64, **h), torch.zeros(4, 2, 64, **h), torch.zeros(64, 128, **h)
+    st = torch.tensor([0, 4], dtype=torch.int32, device=cuda)
+    x = torch.zeros(4, 64, **h)
+    for bad in (k.float(), k.cpu(), k[:3], k[..., :32], k.transpose(0, 1), k[:1].expand(4, 2, 64)):
+        with pytest.raises(rb.TinyError):
+            rb.prompt_attention(q, bad, k, st, 4)
+        with pytest.raises(rb.TinyError):
+            rb.prompt_attention(q, k, bad, st, 4)
+    for kw in (dict(q_start=st.long()), dict(q_start=st[:1]), dict(max_rows=-1),
+               dict(out=torch.zeros(4, 4, 64, device=cuda, dtype=torch.float64)),
+               dict(out=torch.zeros(4, 8, 64, **h)[:, ::2]), dict(lse=torch.zeros(4, 3, device=cuda))):
+        with pytest.raises(rb.TinyError):
+            rb.prompt_attention(**{**dict(q=q, k=k, v=k, q_start=st, max_rows=4), **kw})
+    for kw in (dict(x=x.float()), dict(w=w.t()), dict(w=w[:32]), dict(bias=torch.zeros(64, **h)),
+               dict(bias=torch.zeros(128, device=cuda)), dict(activation="tanh"),
+               dict(residual=torch.zeros(3, 128, **h)), dict(residual=torch.zeros(1, 128, **h).expand(4, 128)),
+               dict(out=torch.zeros(4, 64, **h)), dict(w=w[:, :60]), dict(x=x[:, 1:9], w=w[:8]),
+               dict(w=torch.zeros(64, 31, **h), activation="swiglu")):
+        with pytest.raises(rb.TinyError):
+            rb.prompt_linear(**{**dict(x=x, w=w), **kw})
+    arena = torch.zeros(4, 2, 16, 64, **h)
+    lens = torch.zeros(1, dtype=torch.int32, device=cuda)
+    kv = rb.paged_kv_from_tensors(arena, arena, torch.zeros((1, 4), dtype=torch.int32, device=cuda), lens)
+    for a in ((lens.long(), 4), (lens.expand(2), 4), (lens, -1), (lens.cpu(), 4)):
+        with pytest.raises(rb.TinyError):
+            rb.batch_tables(kv, *a)
+    with pytest.raises(rb.TinyError):
+        rb.batch_tables(kv, lens, 4, free_start=lens)
+    with pytest.raises(rb.TinyError):
+        rb.batch_tables(kv, lens, 4, out=rb.BatchTables.empty(1, 5, cuda))
+    p, s = torch.zeros(4, dtype=torch.int32, device=cuda), torch.zeros(4, dtype=torch.int64, device=cuda)
+    cos = torch.zeros(8, 32, device=cuda)
+    for kw in (dict(positions=p.long()), dict(slots=p), dict(slots=s[:3]), dict(k=k[:, :1]),
+               dict(v=k.float()), dict(rope=(cos[:, :16], cos)), dict(rope=(cos.half(), cos)),
+               dict(q_out=q[:3]), dict(k_out=q), dict(q=q[..., :32])):
+        with pytest.raises(rb.TinyError):
+            rb.rope_append(**{**dict(kv=kv, q=q, k=k, v=k, positions=p, slots=s), **kw})
+    assert float(arena.abs().sum()) == 0
 
 
 # ---- streams, graphs, repeats -----------------------------------------------------------

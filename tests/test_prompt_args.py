@@ -165,6 +165,7 @@ def lin(x=Q, ldx=64, w=K, ldw=128, bias=None, act=0, res=None, ldr=0, out=O, ldo
     (INVALID_ARGUMENT, dict(out=Q)),
     (INVALID_ARGUMENT, dict(res=O + 256, ldr=128)),     # shifted by a row
     (INVALID_ARGUMENT, dict(res=O, ldr=256)),
+    (INVALID_ARGUMENT, dict(out=K + 256)),              # inside W
 ])
 def test_prompt_linear_refusals(want, kw):
     assert lin(**kw) == want
