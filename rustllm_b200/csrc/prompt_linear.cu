@@ -2,6 +2,13 @@
 // of rows, the matrix product on the 5th-generation tensor cores and everything behind it in
 // its epilogue, so the product never makes a round trip through memory.
 //
+// A persistent grid walks the output tiles: one warp feeds x and W tiles through a ring by TMA,
+// one issues the products into one of two accumulators in tensor memory, eight empty the other
+// one, so the epilogue runs under the next tile's products.  Bound by the tensor pipe (92 % active
+// at 8191 x 4096 x 4096 with bias and residual, 179 us = 1.54 PFLOP/s at first, 229 us back to back
+// under the power limit, where a library product alone takes 235) and by latency for few rows
+// (33 x 768 x 2048: 10 us a call).
+//
 // F16 x [rows, k], W [k, n] row-major (nn/linear.rs:26-27), F32 accumulation and F32 all the
 // way through bias, activation (kernels/silu.metal:38-46 for SwiGLU) and residual, one
 // rounding to F16 at the store.
