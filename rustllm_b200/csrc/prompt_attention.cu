@@ -316,20 +316,22 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 //   warp 8          TMA producer: Q tiles, then K and V tiles through a ring
 //   warps 9, 10     MMA issuers of item 0 / 1
 //   warp 11         scrub (below)
-// K and V arrive in tiles of 128 keys and are used in steps of 128 keys, or of 64 above head size
-// 64, where the accumulators leave less tensor memory.  S = Q K^T of a step sits in tensor memory;
+// K and V arrive in tiles of 128 keys and are used in steps of KS: 64 above head size 64, where the
+// accumulators leave less tensor memory, and for short prompts, whose masked steps cost more than
+// a step's fixed part (heads of 64: 512 prompts of 300 tokens, 389 us in steps of 128 and 287 in
+// steps of 64; 16 of 2048 tokens 215 and 229), else 128.  S = Q K^T of a step sits in tensor memory;
 // its rows are read to registers (and the next step's S is computed over it), exponentiated, and P
 // is written to columns of its own as F16, from where it is the A operand of O += P V, so only V
 // crosses shared memory for the second product.
-//   tensor memory, KS keys a step, PB buffers of P: S_i at [KS i, + KS), P_i[b] at [2 KS +
-//   KS / 2 (PB i + b), + KS / 2), O_i at [512 - DP (2 - i), + DP)
+//   tensor memory: S_i at [KS i, + KS), P_i at [2 KS + KS / 2 i, + KS / 2), O_i at
+//   [512 - DP (2 - i), + DP)
 //
-// Bound by the softmax: a step of 64 keys of two items of head size 128 takes about 1,870 cycles, of
-// which the tensor pipe needs 1,024 and the exponentials 768 of the MUFU's (1,024 without the
-// quarter that goes to the multiply-add pipe), and the rest of the softmax's instructions fill the
-// issue slots.  16384 rows of 32/8 heads of 128: 1.76 ms,
-// 1.25 PFLOP/s (2.07 ms back to back under the power limit); 4 x 4096 rows, heads of 64: 380 us,
-// 720 TFLOP/s; 64 prompts of 1 to 2048 tokens, 15/5 heads of 64 (99.7 GFLOP): 249 us.
+// Bound by the softmax groups' own chain of waits, loads, maximum, exponentials and stores: a step
+// of 64 keys of two items of head size 128 takes about 1,850 cycles, of which the tensor pipe needs
+// 1,024 and the exponentials 768 of the MUFU's (1,024 without the quarter that goes to the
+// multiply-add pipe); 54 % of the issue slots are used.  16384 rows of 32/8 heads of 128: 1.71 ms,
+// 1.29 PFLOP/s; 4 x 4096 rows of 32/8 heads of 64: 368 us, 747 TFLOP/s; 64 prompts of up to 2048
+// tokens, 15/5 heads of 64: 350 us, 560 TFLOP/s.
 //
 // Masked places never reach a result: scores that a row does not see are replaced by -inf before
 // the maximum, and since 0 * inf is not 0, the non-finite entries of every V tile that some row
@@ -340,45 +342,43 @@ constexpr int kTile = 128;
 constexpr int kTcThreads = 384;
 constexpr int kWindow = 1024;    // row tiles a launch schedules (131,072 packed rows)
 
-template <int DP>
+template <int DP, int KSV>
 struct AttCfg {
     static constexpr int BLK = 16384;          // 64 columns x 128 rows, swizzled
     static constexpr int TILE = DP / 64 * BLK; // Q, K or V tile
     static constexpr int QBUF = DP == 64 ? 2 : 1;
     static constexpr int STAGES = DP == 64 ? 8 : 4;
     static constexpr int OFF_KV = 2 * QBUF * TILE;
-    static constexpr int OFF_SEQ = OFF_KV + STAGES * TILE;      // int32 sequence of a tile's first row
-    static constexpr int OFF_HIST = OFF_SEQ + kWindow * 4;      // int32 row tiles of each cost
+    static constexpr int OFF_SEQ = OFF_KV + STAGES * TILE;      // int32 see AttSched::tile_seq
+    static constexpr int OFF_FIRST = OFF_SEQ + kWindow * 4;     // uint32 see AttSched::tile_first
+    static constexpr int OFF_HIST = OFF_FIRST + kWindow * 4;    // int32 row tiles of each cost
     static constexpr int OFF_COST = OFF_HIST + kWindow * 4;     // uint16 key tiles of an entry
     static constexpr int OFF_LIST = OFF_COST + kWindow * 2;     // uint16 entries, longest first
     static constexpr int OFF_OUT = OFF_LIST + kWindow * 2;      // a warp's 32 rows x 64 bytes, x 8
     static constexpr int OFF_BAR = OFF_OUT + 8 * 2048;
-    static constexpr int KS = DP == 64 ? 128 : 64;  // keys of a step
-    static constexpr int SPT = 128 / KS;            // steps of a key tile
-    static constexpr int PB = DP == 64 ? 1 : 2;     // buffers of P
-    static_assert(2 * KS + PB * KS + 2 * DP <= 512, "tensor memory");
+    static constexpr int KS = KSV;        // keys of a step
+    static constexpr int SPT = 128 / KS;  // steps of a key tile
+    static_assert(3 * KS + 2 * DP <= 512, "tensor memory");
     static constexpr int SMEM = OFF_BAR + 512 + 1024;  // + alignment
     static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 };
 
 // Barriers: QF/QE Q tile full / empty, KF/KE ring full / empty, SB V tile of a ring stage ready for
-// the product; of each item: S scores ready, F scores read, P probabilities written, O product done
-// (these two of each buffer of P), E accumulator read; DONE all products.  Both MMA warps give back
-// every K and V tile, whether their item uses it or not, so no role falls more than a phase behind
-// the ring.
-template <int DP>
+// the product; of each item: S scores ready, F scores read, P probabilities written, O product done, E
+// accumulator read; DONE all products.  Both MMA warps give back every K and V tile, whether their
+// item uses it or not, so no role falls more than a phase behind the ring.
+template <int DP, int KSV>
 struct AttBar {
-    using Cfg = AttCfg<DP>;
+    using Cfg = AttCfg<DP, KSV>;
     static constexpr int QF = 0, QE = QF + 2 * Cfg::QBUF, KF = QE + 2 * Cfg::QBUF,
                          KE = KF + Cfg::STAGES, S = KE + Cfg::STAGES, F = S + 2, P = F + 2,
-                         O = P + 2 * Cfg::PB, E = O + 2 * Cfg::PB, SB = E + 2, DONE = SB + Cfg::STAGES,
+                         O = P + 2, E = O + 2, SB = E + 2, DONE = SB + Cfg::STAGES,
                          COUNT = DONE + 1;
     static_assert(COUNT * 8 + 64 <= 512, "barrier area");
 };
 
-// Last sequence whose first row is <= row, among [lo, num_seqs).
-__device__ __forceinline__ int seq_at(const PromptArgs& a, int row, int lo) {
-    int hi = a.num_seqs - 1;
+// Last sequence whose first row is <= row, among [lo, hi].
+__device__ __forceinline__ int seq_at(const PromptArgs& a, int row, int lo, int hi) {
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (__ldg(a.q_start + mid) <= row) lo = mid;
@@ -391,8 +391,7 @@ struct AttUnit {
     int kvh, jlo, jhi;         // key tiles the unit streams
     int head[2], tile[2];      // query head and row tile of each item
     int lo[2], hi[2];          // its steps (lo > hi: no such item)
-    int seq[2];                // sequence of the item's first row
-    bool several[2];           // its rows belong to more than one
+    bool several[2];           // its rows belong to more than one sequence
     bool any_several;
     int first;                 // first visible key of the unit's first row
     __device__ __forceinline__ bool on(int i) const { return lo[i] <= hi[i]; }
@@ -404,7 +403,7 @@ struct AttUnit {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             head[i] = bc(head[i]), tile[i] = bc(tile[i]), lo[i] = bc(lo[i]), hi[i] = bc(hi[i]);
-            seq[i] = bc(seq[i]), several[i] = bc(several[i]);
+            several[i] = bc(several[i]);
         }
     }
     // some row of the unit does not see key tile j whole
@@ -417,10 +416,22 @@ struct AttUnit {
 // range first, heads innermost (they share K and V in L2), dealt to the CTAs in a snake so their
 // sums come out alike.
 struct AttSched {
-    const int32_t* tile_seq;
+    const int32_t* tile_seq;     // of each row tile of the window: sequence of its first row,
+    const uint32_t* tile_first;  // that sequence's first row, and kSeveral if it ends in the tile
     const uint16_t* list;
-    int row_lo, row_hi;        // live rows
-    int tile0, per, total, k;  // window's first tile, units of a list entry
+    int row_lo, row_hi;          // live rows
+    int tile0, tile_end;         // the window's first tile; its live ones end here (relative)
+    int per, total, k;           // units of a list entry
+    static constexpr uint32_t kSeveral = 1u << 31;
+
+    // first row of the sequence of a row of (absolute) tile t
+    __device__ __forceinline__ int row_first(const PromptArgs& a, int t, int row) const {
+        t -= tile0;
+        const uint32_t f = tile_first[t];
+        if (!(f & kSeveral)) return static_cast<int>(f);
+        const int hi = t + 1 < tile_end ? tile_seq[t + 1] : a.num_seqs - 1;
+        return max(__ldg(a.q_start + seq_at(a, row, tile_seq[t], hi)), 0);
+    }
 
     template <int KS>
     __device__ __forceinline__ bool next(const PromptArgs& a, AttUnit& u) {
@@ -454,14 +465,12 @@ struct AttSched {
             u.lo[i] = 1;
             u.hi[i] = 0;
             u.several[i] = false;
-            u.seq[i] = 0;
             if (!in) continue;
-            const int s = tile_seq[tile];
+            const uint32_t f = tile_first[tile];
             const int end = r0 + kTile < row_hi ? r0 + kTile : row_hi;
-            u.seq[i] = s;
-            u.several[i] = __ldg(a.q_start + s + 1) < end;
+            u.several[i] = f >> 31;
             u.any_several |= u.several[i];
-            const int first = max(__ldg(a.q_start + s), 0);
+            const int first = static_cast<int>(f & ~kSeveral);
             u.lo[i] = first / KS;
             u.hi[i] = (end - 1) / KS;
             if (i == 0 || !u.on(0)) u.first = first;
@@ -509,14 +518,14 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 }
 __device__ __forceinline__ bool odd_half(uint32_t bits) { return (bits & 0x7C00u) == 0x7C00u; }
 
-template <int DP>
+template <int DP, int KS>
 __global__ void __launch_bounds__(kTcThreads, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap qmap,
                      const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap, const PromptArgs a, int tile0) {
-    using Cfg = AttCfg<DP>;
-    using B = AttBar<DP>;
-    constexpr int KS = Cfg::KS, SPT = Cfg::SPT, PB = Cfg::PB;
+    using Cfg = AttCfg<DP, KS>;
+    using B = AttBar<DP, KS>;
+    constexpr int SPT = Cfg::SPT;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
@@ -548,10 +557,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     // ---- the work list
     int32_t* tile_seq = reinterpret_cast<int32_t*>(smem + Cfg::OFF_SEQ);
+    uint32_t* tile_first = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_FIRST);
     int32_t* hist = reinterpret_cast<int32_t*>(smem + Cfg::OFF_HIST);
     uint16_t* list = reinterpret_cast<uint16_t*>(smem + Cfg::OFF_LIST);
     uint16_t* cost = reinterpret_cast<uint16_t*>(smem + Cfg::OFF_COST);
-    AttSched sched{tile_seq, list, 0, 0, tile0, 0, 0, 0};
+    AttSched sched{tile_seq, tile_first, list, 0, 0, tile0, 0, 0, 0, 0};
     {
         const int q0 = __ldg(a.q_start), q1 = __ldg(a.q_start + a.num_seqs);
         sched.row_lo = q0 > 0 ? q0 : 0;
@@ -561,6 +571,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int ta = sched.row_lo / kTile - tile0, tb = (sched.row_hi + kTile - 1) / kTile - tile0;
         ta = ta > 0 ? ta : 0;
         tb = tb < kWindow ? tb : kWindow;
+        sched.tile_end = tb;
         const int ea = ta / span, eb = (tb + span - 1) / span;
         const int count = sched.row_hi > sched.row_lo && eb > ea ? eb - ea : 0;
         sched.per = a.kv_heads * (a.pairs == 1 ? a.group / 2 : a.group);
@@ -569,7 +580,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = tid; i < kWindow; i += kTcThreads) hist[i] = 0;
         for (int t = ta + tid; t < tb; t += kTcThreads) {
             const int row = (tile0 + t) * kTile;
-            tile_seq[t] = seq_at(a, row > sched.row_lo ? row : sched.row_lo, 0);
+            const int s = seq_at(a, row > sched.row_lo ? row : sched.row_lo, 0, a.num_seqs - 1);
+            const int end = row + kTile < sched.row_hi ? row + kTile : sched.row_hi;
+            tile_seq[t] = s;
+            tile_first[t] = static_cast<uint32_t>(max(__ldg(a.q_start + s), 0)) |
+                            (__ldg(a.q_start + s + 1) < end ? AttSched::kSeveral : 0u);
         }
         __syncthreads();
         if (!sorted) {
@@ -577,7 +592,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         } else {
             for (int i = tid; i < count; i += kTcThreads) {
                 const int t0 = max((ea + i) * span, ta), t1 = min((ea + i) * span + span, tb) - 1;
-                const int c = tile0 + t1 - max(__ldg(a.q_start + tile_seq[t0]), 0) / kTile;
+                const int first = static_cast<int>(tile_first[t0] & ~AttSched::kSeveral);
+                const int c = tile0 + t1 - first / kTile;
                 cost[i] = static_cast<uint16_t>(c < kWindow ? c : kWindow - 1);
                 atomicAdd(hist + cost[i], 1);
             }
@@ -619,9 +635,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     auto tmem_s = [&](int i) { return tmem + static_cast<uint32_t>(KS * i); };
-    auto tmem_p = [&](int i, int b) {
-        return tmem + static_cast<uint32_t>(2 * KS + KS / 2 * (PB * i + b));
-    };
+    auto tmem_p = [&](int i) { return tmem + static_cast<uint32_t>(2 * KS + KS / 2 * i); };
     auto tmem_o = [&](int i) { return tmem + static_cast<uint32_t>(512 - DP * (2 - i)); };
     auto wait = [&](int b, uint32_t parity) {
         return mbar_wait_bounded(bar(b), parity & 1u, abort_flag, &g_attention_status);
@@ -635,7 +649,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // ---- softmax: thread r of group w owns row r of item w
         const int w = warp >> 2, r = tid & 127;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem_s(w) + lane_base, to = tmem_o(w) + lane_base;
+        const uint32_t ts = tmem_s(w) + lane_base, tp = tmem_p(w) + lane_base,
+                       to = tmem_o(w) + lane_base;
         unsigned char* stage = smem + Cfg::OFF_OUT + warp * 2048;
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
         int step = 0;
@@ -643,23 +658,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_wait_uniform(bar(b), phase & 1, abort_addr, &g_attention_status);
         };
         const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-        while (sched.template next<Cfg::KS>(a, u) && !*abort_flag) {
-            const int lo = w ? u.lo[1] : u.lo[0], hi = w ? u.hi[1] : u.hi[0];
-            const int tile = w ? u.tile[1] : u.tile[0], head = w ? u.head[1] : u.head[0];
-            const int row = tile * kTile + r;  // keys `first` .. row are visible
-            const bool on = lo <= hi;
-            const bool live = on && row >= sched.row_lo && row < sched.row_hi;
-            int first = INT32_MAX;
-            if (live) {
-                const int s0 = w ? u.seq[1] : u.seq[0];
-                const bool several = w ? u.several[1] : u.several[0];
-                first = max(__ldg(a.q_start + (several ? seq_at(a, row, s0) : s0)), 0);
-            }
+        struct Row {  // this thread's row of a unit: keys `first` .. row are visible
+            int lo, hi, head, row, first;
+            bool live;
+        } x, y{};  // the current unit's and the next one's, found before the epilogue's wait
+        auto next = [&]() {
+            if (!sched.template next<Cfg::KS>(a, u)) return false;
+            const int tile = w ? u.tile[1] : u.tile[0];
+            y.lo = w ? u.lo[1] : u.lo[0], y.hi = w ? u.hi[1] : u.hi[0];
+            y.head = w ? u.head[1] : u.head[0];
+            y.row = tile * kTile + r;
+            y.live = y.lo <= y.hi && y.row >= sched.row_lo && y.row < sched.row_hi;
+            y.first = y.live ? sched.row_first(a, tile, y.row) : INT32_MAX;
+            return true;
+        };
+        bool more = next();
+        while (more && !*abort_flag) {
+            x = y;
+            const AttUnit now = u;
+            const int lo = x.lo, hi = x.hi, row = x.row, first = x.first, head = x.head;
+            const bool live = x.live;
             float m = -INFINITY, l = 0.f;
             for (int n = lo; n <= hi; ++n) {
-                const bool ragged = u.ragged(n / SPT);
-                const int pb = step % PB;  // this step's buffer of P
-                const uint32_t tp = tmem_p(w, pb) + lane_base;
+                const bool ragged = now.ragged(n / SPT);
                 await(B::S + w, step);
                 tc_fence_after();
                 float v[KS];
@@ -735,18 +756,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pk[e] = 0u;
                     }
-                    if (c == 0 && step >= PB) {  // the buffer's last product has read it
-                        await(B::O + PB * w + pb, step / PB - 1);
+                    if (c == 0 && step > 0) {  // the last product has read P
+                        await(B::O + w, step - 1);
                         tc_fence_after();
                     }
                     tmem_st16_bits(tp + 16 * c, pk);
                 }
                 l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
                 if (rescale) {  // O is to hold the products before this step
-                    if (PB == 2) {
-                        await(B::O + PB * w + (pb ^ 1), (step - 1) / PB);
-                        tc_fence_after();
-                    }
 #pragma unroll 1
                     for (int c = 0; c < DP / 32; ++c) {
                         float o[32];
@@ -758,12 +775,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(bar(B::P + PB * w + pb));
+                mbar_arrive(bar(B::P + w));
                 ++step;
             }
-            if (!on) continue;
+            more = next();  // while the last product runs
+            if (lo > hi) continue;
             // ---- epilogue
-            await(B::O + PB * w + (step - 1) % PB, (step - 1) / PB);
+            await(B::O + w, step - 1);
             tc_fence_after();
             const bool odd = *odd_flag != 0;
             const float inv = l == 0.f ? 0.f : 1.f / l;  // every score -inf: zeros
@@ -778,9 +796,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int i = 0; i < 32; ++i) o[i] *= inv;
                 if (odd && live) {  // the entries the scrub took out, for the rows that see them
                     const __half* vg = static_cast<const __half*>(a.v) +
-                                       static_cast<int64_t>(u.kvh) * a.head_dim + c * 32;
+                                       static_cast<int64_t>(now.kvh) * a.head_dim + c * 32;
                     for (int key = first; key <= row; ++key) {
-                        if (!u.ragged(key / kTile)) {
+                        if (!now.ragged(key / kTile)) {
                             key |= kTile - 1;  // to the tile's end
                             continue;
                         }
@@ -933,21 +951,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const bool mine = n >= lo && n <= hi;
                 if (sub == 0) await(B::SB + stage_of(x), x / Cfg::STAGES);
                 if (mine) {
-                    await(B::P + PB * i + prods % PB, prods / PB);
+                    await(B::P + i, prods);
                     // the accumulator still holds this item's previous unit
                     if (n == lo && units > 0) await(B::E + i, units - 1);
                     tc_fence_after();
                 }
                 const uint32_t va = sbase + Cfg::OFF_KV + stage_of(x) * Cfg::TILE + sub * KS * 128;
                 const uint64_t vd = sw128_desc(va, Cfg::BLK, 1024);
-                const uint32_t d = tmem_o(i), p = tmem_p(i, prods % PB);
+                const uint32_t d = tmem_o(i), p = tmem_p(i);
                 if (leader) {
                     if (mine) {
 #pragma unroll
                         for (int kk = 0; kk < KS / 16; ++kk)
                             tc_mma_ts(d, p + 8u * kk, vd + kk * (2048 >> 4), IDESC_PV,
                                       n > lo || kk > 0);
-                        tc_commit(bar(B::O + PB * i + prods % PB));
+                        tc_commit(bar(B::O + i));
                     }
                     if (sub == SPT - 1) tc_commit(bar(B::KE + stage_of(x)));
                 }
@@ -1025,9 +1043,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
-template <int DP>
+template <int DP, int KS>
 int launch_tc(PromptArgs a, cudaStream_t s) {
-    using Cfg = AttCfg<DP>;
+    using Cfg = AttCfg<DP, KS>;
     CUtensorMap qmap, kmap, vmap;
     if (int st = make_map_heads(&qmap, a.q, a.head_dim, a.q_heads, a.rows, a.q_stride * 2, kTile))
         return st;
@@ -1040,7 +1058,7 @@ int launch_tc(PromptArgs a, cudaStream_t s) {
     TMLLM_CUDA_TRY(cudaGetDevice(&dev));
     const uint64_t bit = dev < 64 ? (1ull << dev) : 0;
     if (!bit || !(opted.load(std::memory_order_relaxed) & bit)) {
-        TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_tc_kernel<DP>,
+        TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_tc_kernel<DP, KS>,
                                             cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
         opted.fetch_or(bit, std::memory_order_relaxed);
     }
@@ -1053,7 +1071,7 @@ int launch_tc(PromptArgs a, cudaStream_t s) {
         // one item a unit while that still leaves SMs idle
         a.pairs = items <= sms ? 0 : a.group % 2 == 0 ? 1 : 2;
         const int64_t ctas = items < sms ? items : sms;
-        prompt_tc_kernel<DP><<<static_cast<unsigned>(ctas), kTcThreads, Cfg::SMEM, s>>>(
+        prompt_tc_kernel<DP, KS><<<static_cast<unsigned>(ctas), kTcThreads, Cfg::SMEM, s>>>(
             qmap, kmap, vmap, a, static_cast<int>(t0));
         TMLLM_LAUNCH_TRY();
     }
@@ -1159,7 +1177,11 @@ int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, c
                     kv_stride % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) &&
                     aligned16(out) && q_stride < (int64_t{1} << 38) && kv_stride < (int64_t{1} << 38);
     if (!tc) return launch_fma_d<__half>(a, s);
-    return head_dim <= 64 ? launch_tc<64>(a, s) : launch_tc<128>(a, s);
+    if (head_dim > 64) return launch_tc<128, 64>(a, s);
+    // (see KS at the kernel; 32 prompts of 1024 tokens of 15/5 heads of 64: 138 us in steps of 128,
+    // 143 of 64; 64 of 1 to 1500 tokens 233 and 219)
+    if (rows < 1024 * static_cast<int64_t>(num_seqs)) return launch_tc<64, 64>(a, s);
+    return launch_tc<64, 128>(a, s);
 }
 
 }  // extern "C"

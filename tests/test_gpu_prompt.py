@@ -381,6 +381,20 @@ def test_prompt_attention_long(cuda):
     attention_case(cuda, [1500], 2, 1, 128, seed=2)
 
 
+@pytest.mark.parametrize("lens", [[1], [129], [255, 1, 257], [0, 0, 5, 0], [1] * 40, [70, 200, 300]])
+@pytest.mark.parametrize("hq,hkv,d", [(6, 2, 64), (3, 1, 64), (2, 2, 40)])
+def test_prompt_attention_few_long_sequences(cuda, lens, hq, hkv, d):
+    """Room for 1024 rows a sequence: heads up to 64 go in steps of 128 keys instead of 64."""
+    attention_case(cuda, lens, hq, hkv, d, seed=d, lead=3, pad=1024 * len(lens) - sum(lens))
+
+    def spoil(q, k, v, starts):
+        end = starts[-1]
+        k[end:], v[end:], q[end:] = math.nan, math.nan, math.nan
+        k[:3], v[:3] = math.nan, math.inf
+        v[end - 1] = math.inf
+    attention_case(cuda, lens, hq, hkv, d, seed=d, lead=3, pad=1024 * len(lens), spoil=spoil)
+
+
 def test_prompt_attention_many_rows(cuda):
     """More packed rows than one launch schedules (131,072), tiles shared by two or three
     sequences, and one sequence across the border."""
