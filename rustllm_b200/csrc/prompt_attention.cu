@@ -331,7 +331,7 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 // 1,024 and the exponentials 768 of the MUFU's (1,024 without the quarter that goes to the
 // multiply-add pipe); 54 % of the issue slots are used.  16384 rows of 32/8 heads of 128: 1.71 ms,
 // 1.29 PFLOP/s; 4 x 4096 rows of 32/8 heads of 64: 368 us, 747 TFLOP/s; 64 prompts of up to 2048
-// tokens, 15/5 heads of 64: 350 us, 560 TFLOP/s.
+// tokens, 15/5 heads of 64: 350 us, 437 TFLOP/s.
 //
 // Masked places never reach a result: scores that a row does not see are replaced by -inf before
 // the maximum, and since 0 * inf is not 0, the non-finite entries of every V tile that some row
@@ -783,7 +783,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ---- epilogue
             await(B::O + w, step - 1);
             tc_fence_after();
-            const bool odd = *odd_flag != 0;
             const float inv = l == 0.f ? 0.f : 1.f / l;  // every score -inf: zeros
             const int64_t orow = (live ? row : 0) * a.out_stride +
                                  static_cast<int64_t>(head) * a.head_dim;
@@ -794,22 +793,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tmem_ld32(to + c * 32, o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] *= inv;
-                if (odd && live) {  // the entries the scrub took out, for the rows that see them
-                    const __half* vg = static_cast<const __half*>(a.v) +
-                                       static_cast<int64_t>(now.kvh) * a.head_dim + c * 32;
-                    for (int key = first; key <= row; ++key) {
-                        if (!now.ragged(key / kTile)) {
-                            key |= kTile - 1;  // to the tile's end
-                            continue;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if (c * 32 + i >= a.head_dim) continue;
-                            const __half hv = vg[key * a.kv_stride + i];
-                            if (odd_half(__half_as_ushort(hv))) o[i] += __half2float(hv);
-                        }
-                    }
-                }
                 if (a.out_f32) {
                     if (!live) continue;
 #pragma unroll
@@ -847,12 +830,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 __syncwarp();
             }
-            __syncwarp();
             tc_fence_before();
             mbar_arrive(bar(B::E + w));
             if (a.lse && live)
                 a.lse[static_cast<int64_t>(row) * a.q_heads + head] =
-                    ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2;
+                    ((m == -INFINITY ? 0.f : m) + __log2f(l)) * kLn2;
+        }
+        // ---- the non-finite values that the scrub took out, added to the stored rows that see
+        // them: all units once more, here and not in the epilogue, where the mere code of this
+        // rare case cost instruction fetches (512 prompts of 300 tokens, 9/3 heads of 64: 290 us,
+        // 272 with it here)
+        if (*odd_flag) {
+            __syncwarp();  // rows are stored by whichever lanes
+            sched.k = 0;
+            while (next()) {
+                if (!y.live) continue;
+                const __half* vg = static_cast<const __half*>(a.v) +
+                                   static_cast<int64_t>(u.kvh) * a.head_dim;
+                const int64_t orow = y.row * a.out_stride +
+                                     static_cast<int64_t>(y.head) * a.head_dim;
+                for (int key = y.first; key <= y.row; ++key) {
+                    if (!u.ragged(key / kTile)) {
+                        key |= kTile - 1;  // to the tile's end
+                        continue;
+                    }
+                    for (int i = 0; i < a.head_dim; ++i) {
+                        const __half hv = vg[key * a.kv_stride + i];
+                        if (!odd_half(__half_as_ushort(hv))) continue;
+                        if (a.out_f32) {
+                            static_cast<float*>(a.out)[orow + i] += __half2float(hv);
+                        } else {
+                            __half* o = static_cast<__half*>(a.out) + orow + i;
+                            *o = __float2half(__half2float(*o) + __half2float(hv));
+                        }
+                    }
+                }
+            }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
