@@ -44,8 +44,9 @@ def _on(device: torch.device, *ts) -> None:
     must never reach a kernel."""
     if device.type != "cuda":
         raise _lib.InvalidArgument(f"tensors must live on a CUDA device, got one on {device}")
+    index = device.index
     for t in ts:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:  # (-1 on the host)
             raise _lib.InvalidArgument(f"tensors must live on {device}, got one on {t.device}")
 
 
@@ -165,8 +166,9 @@ def rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if d != kv.head_dim:
         raise _lib.ModelFormat(f"the cache holds heads of {kv.head_dim}, got {d}")
     dtype = q.dtype
-    if dtype_code(dtype) != kv.dtype or any(
-            t is not None and t.dtype != dtype for t in (k, v, q_out, k_out)):
+    if dtype_code(dtype) != kv.dtype or k.dtype != dtype or v.dtype != dtype or (
+            q_out is not None and q_out.dtype != dtype) or (
+            k_out is not None and k_out.dtype != dtype):
         raise _lib.UnsupportedDType("q, k, v and the cache must have one dtype")
     qs, ks = _stride(q, hq, d, "q"), _stride(k, hkv, d, "k")
     if _stride(v, hkv, d, "v") != ks:
