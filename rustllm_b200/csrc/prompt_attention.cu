@@ -47,33 +47,57 @@ __device__ __forceinline__ int seq_rows(const PromptArgs& a, int s, int64_t* row
 }
 
 // ---- CUDA-core form: any type and head size up to 256 -----------------------------------
-// One CTA per (16 RT query rows, query head, sequence), 256 threads; thread (ty, tx) holds RT rows
-// from RT ty on of S (columns tx + 16 c of a tile of 64 keys) and of O (columns 4 tx + 64 c ..).  DP: head size
-// rounded up to 64 / 128 / 256.  Both products run on packed F32 pairs (two multiply-adds an
-// instruction) out of 16-byte shared-memory reads, 64 multiply-adds per 8 reads; with F32 rows
-// on the 16-byte grid the next K and V tiles are copied while this one is computed (DP <= 128).
-// Bound by the F32 multiply-add rate at long prompts, by latency at short ones.
+// One CTA per (TT / 16 RT query rows, query head, sequence), TEAMS teams of TT threads that take
+// every TEAMS-th tile of keys each and are joined at the end.  Thread (ty, tx) of a team holds RT
+// rows from RT ty on of S (columns tx + 16 c of a tile of 64 keys) and of O (columns 4 tx + 64 c
+// on).  DP: head size rounded up to 64 / 128 / 256.  Both products run on packed F32 pairs (two
+// multiply-adds an instruction) out of 16-byte shared-memory reads: 8 RT multiply-add pairs for
+// RT + 4 reads of 4 cycles each, which is what bounds it at long prompts (4096 tokens, 8 / 2 heads
+// of 128: 950 us, 36 TFLOP/s; 64 x 700 tokens, 9 / 3 heads of 64: 1080 us, 33), so few threads with
+// many rows each; at short ones the chain of a CTA's tiles does, so a second team.  With F32 rows
+// on the 16-byte grid K and V are copied asynchronously, and a single team (DP <= 128) copies the
+// next tile while this one is computed.
 constexpr int kFmaTile = 64;  // keys
 
-template <int DP, int RT>
+template <int DP, int RT, int TT, int TEAMS>
 struct FmaCfg {
-    static constexpr int ROWS = 16 * RT;
+    static constexpr int ROWS = TT / 16 * RT;
     static constexpr int LD = DP + 4;  // pitch of Q and K: rows 16 bytes apart in the banks
-    static constexpr int BUFS = DP <= 128 ? 2 : 1;
+    static constexpr int BUFS = TEAMS == 1 && DP <= 128 ? 2 : 1;  // of each team
     static constexpr int KV = kFmaTile * (LD + DP);  // floats of a K and a V tile
     static constexpr int LP = kFmaTile + 4;
-    static constexpr int SMEM = (ROWS * LD + BUFS * KV + ROWS * LP) * 4;
+    static constexpr int PS = ROWS * LP;
+    static constexpr int SMEM = (ROWS * LD + TEAMS * (BUFS * KV + PS)) * 4;
+    // a team's results fit where its tiles were
+    static_assert(TT * RT * (DP / 16 + 2) <= BUFS * KV, "merge");
 };
 
-template <typename T, int DP, int RT>
-__global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int row_tiles,
-                                                         int async) {
-    using Cfg = FmaCfg<DP, RT>;
+// Barrier `id` of `threads` threads, and whether one of them has x.
+template <int THREADS>
+__device__ __forceinline__ bool barrier_or(int id, bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(static_cast<uint32_t>(x)), "r"(id), "n"(THREADS)
+        : "memory");
+    return any != 0;
+}
+
+template <typename T, int DP, int RT, int TT, int TEAMS>
+__global__ void __launch_bounds__(TT * TEAMS) prompt_fma_kernel(const PromptArgs a, int row_tiles,
+                                                                 int async) {
+    using Cfg = FmaCfg<DP, RT, TT, TEAMS>;
     constexpr int ROWS = Cfg::ROWS, LD = Cfg::LD, LP = Cfg::LP, CG = DP / 64;
     extern __shared__ __align__(16) float fsm[];
     float* qs = fsm;                          // [ROWS][LD]
-    float* kv0 = qs + ROWS * LD;              // [BUFS]: K [64][LD], V [64][DP]
-    float* ps = kv0 + Cfg::BUFS * Cfg::KV;    // [ROWS][LP]
+    const int team = TEAMS == 1 ? 0 : threadIdx.x / TT;
+    float* kv0 = qs + ROWS * LD + team * (Cfg::BUFS * Cfg::KV + Cfg::PS);  // [BUFS]: K [64][LD],
+                                                                           // V [64][DP]
+    float* ps = kv0 + Cfg::BUFS * Cfg::KV;                                 // [ROWS][LP]
     const int64_t hb = static_cast<int64_t>(a.q_heads) * a.num_seqs;
     const int tile = row_tiles - 1 - static_cast<int>(blockIdx.x / hb);
     const int h = static_cast<int>(blockIdx.x % hb) % a.q_heads;
@@ -83,7 +107,7 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
     const int q_lo = tile * ROWS;
     if (q_lo >= n) return;
     const int kvh = h / a.group, D = a.head_dim;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int tid = threadIdx.x % TT, tx = tid & 15, ty = tid >> 4;
     const T* qg = static_cast<const T*>(a.q) + (row0 + q_lo) * a.q_stride +
                   static_cast<int64_t>(h) * D;
     const T* kg = static_cast<const T*>(a.k) + row0 * a.kv_stride + static_cast<int64_t>(kvh) * D;
@@ -94,7 +118,7 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
         float* ks = kv0 + buf * Cfg::KV;
         float* vs = ks + kFmaTile * LD;
         if (async) {
-            for (int i = tid; i < kFmaTile * (DP / 4); i += 256) {
+            for (int i = tid; i < kFmaTile * (DP / 4); i += TT) {
                 const int r = i / (DP / 4), c = (i % (DP / 4)) * 4;
                 const bool in = j0 + r < q_hi && c < D;  // D is a multiple of 4 here
                 const int64_t off = in ? static_cast<int64_t>(j0 + r) * a.kv_stride + c : 0;
@@ -103,7 +127,7 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
             }
             cp_async_commit();
         } else {
-            for (int i = tid; i < kFmaTile * DP; i += 256) {
+            for (int i = tid; i < kFmaTile * DP; i += TT) {
                 const int r = i / DP, c = i % DP;
                 const bool in = j0 + r < q_hi && c < D;
                 const int64_t off = static_cast<int64_t>(j0 + r) * a.kv_stride + c;
@@ -112,8 +136,9 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
             }
         }
     };
-    load(0, 0);
-    for (int i = tid; i < ROWS * DP; i += 256) {
+    constexpr int STRIDE = TEAMS * kFmaTile;  // between a team's tiles
+    if (team * kFmaTile < q_hi) load(team * kFmaTile, 0);
+    for (int i = threadIdx.x; i < ROWS * DP; i += TT * TEAMS) {
         const int r = i / DP, c = i % DP;
         qs[r * LD + c] = (q_lo + r < n && c < D) ? to_f32<T>(qg[r * a.q_stride + c]) : 0.f;
     }
@@ -126,24 +151,29 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
 #pragma unroll
         for (int c = 0; c < 2 * CG; ++c) o[i][c] = make_float2(0.f, 0.f);
     }
+    if (TEAMS > 1) __syncthreads();  // Q
+    auto team_sync = [&]() {
+        if (TEAMS == 1) __syncthreads();
+        else asm volatile("barrier.cta.sync %0, %1;" ::"r"(1 + team), "n"(TT) : "memory");
+    };
     int buf = 0;
-    for (int j0 = 0; j0 < q_hi; j0 += kFmaTile) {
-        const bool ahead = Cfg::BUFS == 2 && async && j0 + kFmaTile < q_hi;
+    for (int j0 = team * kFmaTile; j0 < q_hi; j0 += STRIDE) {
+        const bool ahead = Cfg::BUFS == 2 && async && j0 + STRIDE < q_hi;
         if (ahead) {
-            load(j0 + kFmaTile, buf ^ 1);
+            load(j0 + STRIDE, buf ^ 1);
             cp_async_wait<1>();
         } else {
             cp_async_wait<0>();
         }
-        __syncthreads();
+        team_sync();
         const float* ks = kv0 + buf * Cfg::KV;
         const float* vs = ks + kFmaTile * LD;
         const bool diag = j0 + kFmaTile > q_lo;
         // 0 * inf is not 0: a diagonal tile with non-finite values takes the masked product
         bool odd = false;
         if (diag) {
-            for (int i = tid; i < kFmaTile * DP; i += 256) odd |= !(fabsf(vs[i]) < INFINITY);
-            odd = __syncthreads_or(odd);
+            for (int i = tid; i < kFmaTile * DP; i += TT) odd |= !(fabsf(vs[i]) < INFINITY);
+            odd = TEAMS == 1 ? __syncthreads_or(odd) != 0 : barrier_or<TT>(1 + team, odd);
         }
         float2 s2[RT][4];
 #pragma unroll
@@ -237,11 +267,43 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
                     }
                 }
         }
-        __syncthreads();  // the tiles are done with
+        team_sync();  // the tiles are done with
         if (ahead) {
             buf ^= 1;
-        } else if (j0 + kFmaTile < q_hi) {
-            load(j0 + kFmaTile, buf);
+        } else if (j0 + STRIDE < q_hi) {
+            load(j0 + STRIDE, buf);
+        }
+    }
+    if (TEAMS > 1) {  // the first team joins the others' rows to its own
+        float2* part = reinterpret_cast<float2*>(kv0);  // [RT (2 CG + 1)][TT]
+        constexpr int W = 2 * CG + 1;
+        if (team > 0) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+#pragma unroll
+                for (int c = 0; c < 2 * CG; ++c) part[(i * W + c) * TT + tid] = o[i][c];
+                part[(i * W + 2 * CG) * TT + tid] = make_float2(m[i], l[i]);
+            }
+        }
+        __syncthreads();
+        if (team > 0) return;
+#pragma unroll
+        for (int t = 1; t < TEAMS; ++t) {
+            part = reinterpret_cast<float2*>(kv0 + t * (Cfg::BUFS * Cfg::KV + Cfg::PS));
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const float2 ml = part[(i * W + 2 * CG) * TT + tid];
+                const float mn = fmaxf(m[i], ml.x), base = mn == -INFINITY ? 0.f : mn;
+                const float own = exp2f(m[i] - base), its = exp2f(ml.x - base);
+                l[i] = l[i] * own + ml.y * its;
+                m[i] = mn;
+#pragma unroll
+                for (int c = 0; c < 2 * CG; ++c) {
+                    const float2 x = part[(i * W + c) * TT + tid];
+                    o[i][c] = make_float2(fmaf(x.x, its, o[i][c].x * own),
+                                          fmaf(x.y, its, o[i][c].y * own));
+                }
+            }
         }
     }
 #pragma unroll
@@ -267,33 +329,40 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const PromptArgs a, int
     }
 }
 
-template <typename T, int DP, int RT>
+template <typename T, int DP, int RT, int TT, int TEAMS>
 int launch_fma_rows(const PromptArgs& a, cudaStream_t s) {
-    const int row_tiles = (a.max_rows + 16 * RT - 1) / (16 * RT);
+    const int row_tiles = (a.max_rows + FmaCfg<DP, RT, TT, TEAMS>::ROWS - 1) / FmaCfg<DP, RT, TT, TEAMS>::ROWS;
     int64_t ctas;
     if (!mul_ok(static_cast<int64_t>(row_tiles) * a.q_heads, a.num_seqs, &ctas) ||
         ctas > INT32_MAX)
         return fail(TMLLM_INVALID_SHAPE, "too many prompt tiles");
-    constexpr int smem = FmaCfg<DP, RT>::SMEM;
+    constexpr int smem = FmaCfg<DP, RT, TT, TEAMS>::SMEM;
     static_assert(smem <= 227 * 1024, "shared memory of one CTA");
     const int async = sizeof(T) == 4 && a.head_dim % 4 == 0 && a.kv_stride % 4 == 0 &&
                       aligned16(a.k) && aligned16(a.v);
-    TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_fma_kernel<T, DP, RT>,
+    TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_fma_kernel<T, DP, RT, TT, TEAMS>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    prompt_fma_kernel<T, DP, RT><<<static_cast<unsigned>(ctas), 256, smem, s>>>(a, row_tiles, async);
+    prompt_fma_kernel<T, DP, RT, TT, TEAMS>
+        <<<static_cast<unsigned>(ctas), TT * TEAMS, smem, s>>>(a, row_tiles, async);
     TMLLM_LAUNCH_TRY();
     return TMLLM_OK;
 }
 
-// 64 query rows a CTA read K and V half as often; 32 spread a small batch over more SMs and halve
-// its longest CTA (F32, 270 CTAs of 64 rows over 9 prompts of up to 500 tokens: 53 us against 45;
-// 420 CTAs over 4 x 500 tokens, 12 heads of 64: 81 against 104; 4096 tokens, 8 / 2 heads of 128:
-// 957 us, 36 TFLOP/s, against 1562).
+// 64 query rows a CTA read K and V half as often; 32 spread a small batch over more SMs, and two
+// teams halve its longest CTA (F32, 270 CTAs of 64 rows over 9 prompts of up to 413 tokens, heads
+// of 64: 31 us, 42 with one team of 256 threads; 2 x 500 tokens, 8 / 2 heads of 128: 46 against
+// 61; but 520 CTAs over 4096 tokens, heads of 128: 994 against 949).
 template <typename T, int DP>
 int launch_fma(const PromptArgs& a, cudaStream_t s) {
-    const int64_t ctas = (a.rows / 64 + a.num_seqs) * a.q_heads;
-    return ctas < 2 * device_sm_count() ? launch_fma_rows<T, DP, 2>(a, s)
-                                        : launch_fma_rows<T, DP, 4>(a, s);
+    const bool small = (a.rows / 64 + a.num_seqs) * a.q_heads < 2 * device_sm_count();
+    if constexpr (DP <= 128) {
+        if (small) return launch_fma_rows<T, DP, 4, 128, 2>(a, s);
+        return DP == 64 ? launch_fma_rows<T, 64, 8, 128, 1>(a, s)
+                        : launch_fma_rows<T, DP, 4, 256, 1>(a, s);
+    } else {  // one tile of K and V fills the shared memory
+        return small ? launch_fma_rows<T, DP, 2, 256, 1>(a, s)
+                     : launch_fma_rows<T, DP, 4, 256, 1>(a, s);
+    }
 }
 
 template <typename T>
@@ -840,8 +909,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // them: all units once more, here and not in the epilogue, where the mere code of this
         // rare case cost instruction fetches (512 prompts of 300 tokens, 9/3 heads of 64: 290 us,
         // 272 with it here)
-        if (*odd_flag) {
-            __syncwarp();  // rows are stored by whichever lanes
+        __syncwarp();  // rows are stored by whichever lanes
+        if (__any_sync(FULL, *odd_flag != 0)) {
             sched.k = 0;
             while (next()) {
                 if (!y.live) continue;

@@ -376,6 +376,31 @@ def test_prompt_attention_f32_lengths(cuda):
         attention_case(cuda, lens, 9, 3, 64, torch.float32, seed=3)
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.float32, 40), (torch.float32, 128),
+                                     (torch.float32, 200), (torch.float16, 20), (torch.float16, 136)])
+def test_prompt_attention_cuda_cores_many_heads(cuda, dtype, d):
+    """Enough heads for 64 rows a CTA (32 rows and two teams a CTA otherwise), the keys that rows
+    do not see not finite."""
+    lens = [1, 63, 130, 0, 65, 200]
+    attention_case(cuda, lens, 48, 4, d, dtype, seed=d, pad=3, lead=2)
+
+    def spoil(q, k, v, starts):
+        end = starts[-1]
+        k[end:], v[end:], q[end:], k[:2], v[:2] = (math.nan,) * 5
+        k[end - 30], v[end - 30], v[end - 1] = math.nan, math.inf, -math.inf
+    attention_case(cuda, lens, 48, 4, d, dtype, seed=d + 1, pad=3, lead=2, spoil=spoil)
+
+
+@pytest.mark.parametrize("d", [64, 24, 128])
+@pytest.mark.parametrize("n", [64, 65, 96, 97, 128, 129, 160, 193, 320])
+def test_prompt_attention_cuda_cores_tiles(cuda, d, n):
+    """One sequence ending before, at and behind the tiles of 64 keys that two teams take in turn."""
+    attention_case(cuda, [n], 2, 1, d, torch.float32, seed=n, std=2.0)
+    out = attention_case(cuda, [n, 3], 2, 1, d, torch.float32, seed=n,
+                         spoil=lambda q, k, v, s: (q.abs_(), k[:n - 1].fill_(-math.inf)))
+    assert bool((out[:n - 1] == 0).all()) and bool((out[n - 1] != 0).any())
+
+
 def test_prompt_attention_long(cuda):
     attention_case(cuda, [2000, 100, 1100], 3, 1, 64, seed=1)
     attention_case(cuda, [1500], 2, 1, 128, seed=2)
