@@ -7,11 +7,14 @@
 // one, so the epilogue runs under the next tile's products.  Bound by the tensor pipe (92 % active
 // at 8191 x 4096 x 4096 with bias and residual, 179 us = 1.54 PFLOP/s at first, 229 us back to back
 // under the power limit, where a library product alone takes 235) and by latency for few rows
-// (33 x 768 x 2048: 10 us a call).
+// (33 x 768 x 2048: 6.4 us in a graph, 10 us a call), where K is split over the CTAs of a cluster
+// if it is long (33 x 4096 x 64: 5.9 us instead of 16.9, library product 6.7; 33 x 4096 x 4096: 12.6
+// instead of 18.5, library 9.7).
 //
 // F16 x [rows, k], W [k, n] row-major (nn/linear.rs:26-27), F32 accumulation and F32 all the
 // way through bias, activation (kernels/silu.metal:38-46 for SwiGLU) and residual, one
 // rounding to F16 at the store.
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -32,7 +35,8 @@ enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_SWI
 struct LinArgs {
     const __half* bias;
     const __half* residual;
-    int64_t ld_res;
+    __half* out;
+    int64_t ld_res, ld_out;
     int32_t rows, k, n, act;
     int32_t m_tiles, n_tiles, tiles, group_m;
 };
@@ -60,22 +64,34 @@ __device__ __forceinline__ float relu(float x) { return x > 0.f ? x : (x <= 0.f 
 // BN: accumulator columns of a tile; with GATED half of them are gate and half up columns.
 // PAIR: the two CTAs of a cluster share a tile of 256 rows, each with its 128 rows of A and half
 // the columns of W in shared memory.
-template <int BN, bool GATED, bool PAIR = false>
+// SPLIT > 1: the SPLIT CTAs of a cluster take a part of K of one tile each; every CTA then gets
+// the others' sums of its share of the columns and stores those.
+template <int BN, bool GATED, bool PAIR = false, int SPLIT = 1>
 struct LinCfg {
     static constexpr int ON = GATED ? BN / 2 : BN;  // output columns of a tile
     static constexpr int A_BYTES = kM * kK * 2;
     static constexpr int BC = PAIR ? BN / 2 : BN;  // columns of W in this CTA
     static constexpr int B_BYTES = BC * kK * 2;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
-    // output staging: every epilogue warp has two buffers of 32 rows x 32 columns
+    // output staging: every epilogue warp has two buffers of 32 rows x 32 columns; with a split K
+    // the sums of this CTA's share of the columns from every CTA instead
+    static constexpr int OUT_BYTES = SPLIT > 1 ? kM * BN * 4 : kEpiWarps * 2 * 2048;
+    static constexpr int RING = 229376 - OUT_BYTES;
+    static constexpr int STAGES = RING / STAGE < 8 ? RING / STAGE : 8;
     static constexpr int OFF_OUT = STAGES * STAGE;
-    static constexpr int OFF_BIAS = OFF_OUT + kEpiWarps * 2 * 2048;
+    static constexpr int OFF_BIAS = OFF_OUT + OUT_BYTES;
     static constexpr int OFF_BAR = OFF_BIAS + 2 * BN * 2;  // bias as F16
     static constexpr int SMEM = OFF_BAR + 512 + 1024;  // + alignment
     static constexpr int ACC = BN <= 64 ? 64 : BN <= 128 ? 128 : 256;  // columns apart
     static constexpr int TMEM_COLS = 2 * ACC;                          // two accumulators
     static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
+    static constexpr int SHARE = ON / SPLIT;  // output columns of a CTA
+    static_assert(SHARE % 8 == 0, "16 bytes of a row");
+    // 8 accumulator columns 8 i .. among those of the CTA that stores them
+    static __device__ __forceinline__ int chunk(int i) {
+        const int up = GATED && i * 8 >= ON;
+        return up * (SHARE / 8) + (i - up * (ON / 8)) % (SHARE / 8);
+    }
 };
 
 // Tile `t`: groups of group_m row tiles sweep the columns together, so a wave's A and W tiles
@@ -89,13 +105,14 @@ __device__ __forceinline__ void tile_of(const LinArgs& a, int t, int& m, int& n)
     n = r / gm;
 }
 
-template <int BN, bool GATED, bool PAIR>
+template <int BN, bool GATED, bool PAIR, int SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_linear_kernel(const __grid_constant__ CUtensorMap xmap,
                          const __grid_constant__ CUtensorMap wmap,
                          const __grid_constant__ CUtensorMap omap,
                          const __grid_constant__ CUtensorMap rmap, const LinArgs a) {
-    using Cfg = LinCfg<BN, GATED, PAIR>;
+    using Cfg = LinCfg<BN, GATED, PAIR, SPLIT>;
+    static_assert(!PAIR || SPLIT == 1, "one use of the cluster");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
@@ -142,16 +159,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     tc_fence_before();
-    if (PAIR) cluster_sync_all();  // the other CTA's barriers are ready too
+    if (PAIR || SPLIT > 1) cluster_sync_all();  // the other CTAs' barriers are ready too
     else __syncthreads();
     tc_fence_after();
     // the pair walks the tiles together; this CTA has the rows from `row_of` on
     const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
-    const int tile_first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-    const int tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const int share = SPLIT > 1 ? static_cast<int>(cluster_rank()) : 0;  // of K and the columns
+    const int tile_first = blockIdx.x / (PAIR ? 2 : SPLIT);
+    const int tile_step = gridDim.x / (PAIR ? 2 : SPLIT);
     auto row_of = [&](int m) { return PAIR ? (2 * m + rank) * kM : m * kM; };
     const uint32_t tmem = *tmem_slot;
-    const int nk = (a.k + kK - 1) / kK;
+    const int k_steps = (a.k + kK - 1) / kK;  // this CTA's are [k_lo, k_lo + nk)
+    const int k_lo = static_cast<int>(static_cast<int64_t>(k_steps) * share / SPLIT);
+    const int nk = static_cast<int>(static_cast<int64_t>(k_steps) * (share + 1) / SPLIT) - k_lo;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -174,14 +194,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (PAIR) tma_load_2d_pair(dst, map, x, y, fb);
                         else tma_load_2d(dst, map, x, y, fb);
                     };
-                    load(sa, &xmap, kb * kK, row_of(m));
+                    load(sa, &xmap, (k_lo + kb) * kK, row_of(m));
 #pragma unroll
                     for (int c = 0; c < Cfg::BC / 64; ++c) {
                         const int tc = rank * Cfg::BC + c * 64;  // accumulator column
                         const int col = GATED ? (tc < Cfg::ON ? n * Cfg::ON + tc
                                                               : a.n + n * Cfg::ON + tc - Cfg::ON)
                                               : n * BN + tc;
-                        load(sb + c * (64 * kK * 2), &wmap, col, kb * kK);
+                        load(sb + c * (64 * kK * 2), &wmap, col, (k_lo + kb) * kK);
                     }
                 }
             }
@@ -232,6 +252,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_drain(done, 0);
         }
         __syncwarp();
+    } else if (SPLIT > 1 && warp > 1) {
+        // ---- the sums of the others' columns go to them, 8 columns and 32 rows at a time:
+        // [CTA][8 columns][4 of them][row] of 16 bytes
+        const int row = (warp & 3) * 32 + lane;
+        const uint32_t acc = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        mbar_wait_uniform(acc_full(0), 0, smem_u32(const_cast<int*>(abort_flag)), &g_linear_status);
+        tc_fence_after();
+#pragma unroll 1
+        for (int i = (warp - 2) >> 2; i < BN / 8; i += 2) {  // 8 columns of the tile
+            const int o = i * 8 % Cfg::ON, to = o / Cfg::SHARE;  // output column, its CTA
+            if (to == share) continue;
+            float y[8];
+            tmem_ld8(acc + i * 8, y);
+            const uint32_t slot = static_cast<uint32_t>(
+                Cfg::OFF_OUT + ((share * (BN / 8 / SPLIT) + Cfg::chunk(i)) * 2 * kM + row) * 16);
+            const uint32_t dst = cluster_addr(sbase + slot, to);
+            st_cluster(dst, y[0], y[1], y[2], y[3]);
+            st_cluster(dst + kM * 16, y[4], y[5], y[6], y[7]);
+        }
     } else if (warp > 1) {
         // ---- epilogue: a warp owns 32 rows and every other 32 columns of the tile.  It works
         // alone: its rows leave through its own two buffers and bulk stores; the residual
@@ -344,6 +383,68 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     }
     __syncwarp();
+    if (SPLIT > 1) {
+        cluster_sync_all();  // all sums have arrived
+        // ---- this CTA's columns: a thread has one row of every other 8 of them
+        int m, n;
+        tile_of(a, tile_first, m, n);
+        const int row = (warp & 3) * 32 + lane, grow = m * kM + row;
+        const uint32_t acc = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+#pragma unroll 1
+        for (int c = (warp - 2) >> 2; warp > 1 && c < Cfg::SHARE / 8; c += 2) {
+            const int o = share * Cfg::SHARE + c * 8, col = n * Cfg::ON + o;
+            if (col >= a.n) break;  // n is a multiple of 8
+            auto sum = [&](int i, float (&y)[8]) {  // columns 8 i .. of the tile
+                float own[8];
+                tmem_ld8(acc + i * 8, own);
+#pragma unroll
+                for (int q = 0; q < SPLIT; ++q) {  // in order of K, whichever CTA adds
+                    const float4* part = reinterpret_cast<const float4*>(smem + Cfg::OFF_OUT) +
+                                         (q * (BN / 8 / SPLIT) + Cfg::chunk(i)) * 2 * kM + row;
+                    const float4 lo = part[0], hi = part[kM];
+                    const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float v = q == share ? own[e] : x[e];
+                        y[e] = q == 0 ? v : y[e] + v;
+                    }
+                }
+                if (a.bias) {
+                    const __half* b = a.bias + (GATED && i * 8 >= Cfg::ON ? a.n + col : col);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] += __half2float(b[e]);
+                }
+            };
+            float y[8];
+            sum(o / 8, y);
+            if (GATED) {
+                float u[8];
+                sum((Cfg::ON + o) / 8, u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = silu(y[e]) * u[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    y[e] = a.act == ACT_GELU   ? gelu(y[e])
+                           : a.act == ACT_SILU ? silu(y[e])
+                           : a.act == ACT_RELU ? relu(y[e])
+                                               : y[e];
+            }
+            if (grow < a.rows) {
+                if (a.residual) {
+                    float f[8];
+                    Chunk<__half>::unpack(
+                        *reinterpret_cast<const uint4*>(a.residual + grow * a.ld_res + col), f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] += f[e];
+                }
+                *reinterpret_cast<uint4*>(a.out + grow * a.ld_out + col) =
+                    make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]),
+                               pack_half2(y[4], y[5]), pack_half2(y[6], y[7]));
+            }
+            __syncwarp();
+        }
+    }
     tc_fence_before();
     if (PAIR) cluster_sync_all();  // neither CTA leaves while the other one uses its memory
     else __syncthreads();
@@ -369,10 +470,10 @@ inline int64_t time_of(int64_t m_tiles, int64_t n_tiles, int units, int weight, 
     return (m_tiles * n_tiles + units - 1) / units * (weight * ksteps + 1500);
 }
 
-template <int BN, bool GATED, bool PAIR = false>
+template <int BN, bool GATED, bool PAIR = false, int SPLIT = 1>
 int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ldo,
            LinArgs a, cudaStream_t s) {
-    using Cfg = LinCfg<BN, GATED, PAIR>;
+    using Cfg = LinCfg<BN, GATED, PAIR, SPLIT>;
     CUtensorMap xmap, wmap, omap;
     if (int st = make_map(&xmap, x, a.k, a.rows, ldx * 2, kM)) return st;
     if (int st = make_map(&wmap, w, GATED ? 2 * static_cast<int64_t>(a.n) : a.n, a.k, ldw * 2, kK))
@@ -393,7 +494,7 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, in
     TMLLM_CUDA_TRY(cudaGetDevice(&dev));
     const uint64_t bit = dev < 64 ? (1ull << dev) : 0;
     if (!bit || !(opted.load(std::memory_order_relaxed) & bit)) {
-        TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_linear_kernel<BN, GATED, PAIR>,
+        TMLLM_CUDA_TRY(cudaFuncSetAttribute(prompt_linear_kernel<BN, GATED, PAIR, SPLIT>,
                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             Cfg::SMEM));
         opted.fetch_or(bit, std::memory_order_relaxed);
@@ -404,18 +505,18 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, in
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Cfg::SMEM;
     cfg.stream = s;
-    if (PAIR) {
+    if (PAIR || SPLIT > 1) {
         const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
-        cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+        cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * pairs : SPLIT * tiles));
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.x = PAIR ? 2 : SPLIT;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     } else {
         cfg.gridDim = dim3(static_cast<unsigned>(tiles < sms ? tiles : sms));
     }
-    TMLLM_CUDA_TRY(cudaLaunchKernelEx(&cfg, prompt_linear_kernel<BN, GATED, PAIR>, xmap, wmap, omap,
+    TMLLM_CUDA_TRY(cudaLaunchKernelEx(&cfg, prompt_linear_kernel<BN, GATED, PAIR, SPLIT>, xmap, wmap, omap,
                                       rmap, a));
     TMLLM_LAUNCH_TRY();
     return TMLLM_OK;
@@ -475,7 +576,9 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     LinArgs a{};
     a.bias = static_cast<const __half*>(bias);
     a.residual = static_cast<const __half*>(residual);
+    a.out = static_cast<__half*>(out);
     a.ld_res = ldr;
+    a.ld_out = ldo;
     a.rows = rows;
     a.k = k;
     a.n = n;
@@ -487,10 +590,50 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     const int64_t ksteps = (k + 15) / 16;
     const int sms = device_sm_count();
     auto tiles = [&](int on) { return (static_cast<int64_t>(n) + on - 1) / on; };
+    // Few tiles with a long K: the split of K over a cluster with the shortest time, if that is
+    // shorter.  Handing the sums round costs 6 units a column and CTA, and the first 6 to 8 K steps
+    // of a CTA are in flight together, so shorter parts gain nothing (33 x 4096 x 512: 17.4 us in
+    // one part, 10.8, 7.9, 6.5 in 2, 4, 8; 33 x 512 x 512: 4.8 in one, 5.3 in 2).
+    auto split_time = [&](int on, int bn, int weight, int split) {
+        const int64_t count = mt * tiles(on);
+        // 148 SMs hold 74 clusters of 2, 33 of 4, 15 of 8 at once
+        if (count * 148 > sms * (split == 2 ? 74 : split == 4 ? 33 : 15) ||
+            (k + kK - 1) / kK < (bn == 64 ? 6 : 8) * split)
+            return INT64_MAX;
+        return time_of(1, 1, 1, weight, (ksteps + split - 1) / split) + 400 +
+               int64_t{6} * bn * (split - 1);
+    };
+    struct Split {
+        int64_t time;
+        int which;
+    } sp{INT64_MAX, 0};
+    auto offer = [&](int64_t time, int which) {
+        if (time < sp.time) sp = {time, which};
+    };
+    if (activation == ACT_SWIGLU) {
+        for (int i = 2; i <= 8; i *= 2) offer(split_time(64, 128, 170, i), i);
+    } else {
+        for (int i = 2; i <= 8; i *= 2) offer(split_time(64, 64, 130, i), i);
+        for (int i = 2; i <= 8; i *= 2) offer(split_time(128, 128, 170, i), 16 + i);
+    }
+    auto launch_split = [&]() {
+        switch (activation == ACT_SWIGLU ? 32 + sp.which : sp.which) {
+            case 2: return launch<64, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
+            case 4: return launch<64, false, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
+            case 8: return launch<64, false, false, 8>(x, ldx, w, ldw, out, ldo, a, s);
+            case 18: return launch<128, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
+            case 20: return launch<128, false, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
+            case 24: return launch<128, false, false, 8>(x, ldx, w, ldw, out, ldo, a, s);
+            case 34: return launch<128, true, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
+            case 36: return launch<128, true, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
+            default: return launch<128, true, false, 8>(x, ldx, w, ldw, out, ldo, a, s);
+        }
+    };
     if (activation == ACT_SWIGLU) {
         const int64_t t256 = time_of(mt, tiles(128), sms, 256, ksteps);
         const int64_t t128 = time_of(mt, tiles(64), sms, 170, ksteps);
         const int64_t pair = time_of(mp, tiles(128), sms / 2, 224, ksteps);
+        if (sp.time < std::min(std::min(pair, t256), t128)) return launch_split();
         if (pair < t256 && pair < t128)
             return launch<256, true, true>(x, ldx, w, ldw, out, ldo, a, s);
         return t256 <= t128 ? launch<256, true>(x, ldx, w, ldw, out, ldo, a, s)
@@ -503,6 +646,7 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     int best = 0;
     for (int i = 1; i < 5; ++i)
         if (times[i] < times[best]) best = i;
+    if (sp.time < times[best]) return launch_split();
     switch (best) {
         case 0: return launch<64, false>(x, ldx, w, ldw, out, ldo, a, s);
         case 1: return launch<128, false>(x, ldx, w, ldw, out, ldo, a, s);

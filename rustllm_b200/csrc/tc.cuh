@@ -256,6 +256,12 @@ __device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t a_desc, ui
         : "memory");
 }
 // Arrives on the barrier at `bar`'s offset in both CTAs once this thread's products are done.
+// 16 bytes to shared memory of a CTA of the cluster (16-byte aligned, from cluster_addr).
+__device__ __forceinline__ void st_cluster(uint32_t addr, float x, float y, float z, float w) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y),
+                 "f"(z), "f"(w)
+                 : "memory");
+}
 __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
@@ -283,6 +289,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
         : "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// 8 columns, the same way.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+          "=f"(v[7])
+        : "r"(taddr)
+        : "memory");
 }
 // All 128 F32 columns of this thread's lane in one load (and its wait).
 __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {

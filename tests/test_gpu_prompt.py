@@ -530,6 +530,37 @@ def test_prompt_linear_pairs_of_ctas(cuda, rows, k, n):
     linear_case(cuda, rows, k, n // 2 + 8 - n // 2 % 8, "swiglu", bias=True, residual=True, seed=3)
 
 
+@pytest.mark.parametrize("rows,k,n,act", [
+    (33, 4096, 64, "none"), (1, 4104, 88, "gelu"), (130, 4096, 512, "relu"), (33, 4040, 1000, "silu"),
+    (512, 1024, 1024, "none"), (256, 4096, 4096, "gelu"), (33, 4096, 4096, "none"),
+    (33, 8192, 1016, "silu"), (33, 4096, 2048, "swiglu"), (9, 2048, 2560, "swiglu"),
+    (70, 4104, 488, "swiglu"), (129, 520, 40, "none")])
+def test_prompt_linear_long_products_of_few_tiles(cuda, rows, k, n, act):
+    """K split over 2, 4 and 8 CTAs, columns and K that no part divides."""
+    linear_case(cuda, rows, k, n, act, bias=True, residual=True, seed=rows, xpad=8, opad=8, wpad=16)
+    linear_case(cuda, rows, k, n, act, seed=rows + 1)
+    linear_case(cuda, rows, k, n, act, residual=True, seed=rows + 2, inplace=True)
+
+
+def test_prompt_linear_split_again_and_captured(cuda):
+    """The same bits every time, also from a replayed graph beside another stream's calls."""
+    g = gen(cuda, 5)
+    x, w = randn(g, 40, 4096), randn(g, 4096, 600, std=1 / 64)
+    want = rb.prompt_linear(x, w, activation="gelu")
+    out, other = torch.empty_like(want), torch.empty_like(want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rb.prompt_linear(x, w, activation="gelu", out=out)
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        graph.replay()
+        with torch.cuda.stream(side):
+            rb.prompt_linear(x, w, activation="gelu", out=other)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(other, want) and rb.prompt_status() == 0
+
+
 def test_prompt_linear_non_finite_rows_stay_apart(cuda):
     """NaN in one row of x, or past k in its buffer, reaches that row alone."""
     x = torch.ones(200, 128, dtype=torch.float16, device=cuda)
