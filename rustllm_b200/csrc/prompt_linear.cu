@@ -74,8 +74,9 @@ struct LinCfg {
     static constexpr int B_BYTES = BC * kK * 2;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     // output staging: every epilogue warp has two buffers of 32 rows x 32 columns; with a split K
-    // the sums of this CTA's share of the columns from every CTA instead
-    static constexpr int OUT_BYTES = SPLIT > 1 ? kM * BN * 4 : kEpiWarps * 2 * 2048;
+    // the sums of this CTA's share of the columns from every other CTA instead
+    static constexpr int OUT_BYTES =
+        SPLIT > 1 ? kM * (BN / SPLIT) * 4 * (SPLIT - 1) : kEpiWarps * 2 * 2048;
     static constexpr int RING = 229376 - OUT_BYTES;
     static constexpr int STAGES = RING / STAGE < 8 ? RING / STAGE : 8;
     static constexpr int OFF_OUT = STAGES * STAGE;
@@ -265,8 +266,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (to == share) continue;
             float y[8];
             tmem_ld8(acc + i * 8, y);
+            const int from = share < to ? share : share - 1;  // among the CTAs that send there
             const uint32_t slot = static_cast<uint32_t>(
-                Cfg::OFF_OUT + ((share * (BN / 8 / SPLIT) + Cfg::chunk(i)) * 2 * kM + row) * 16);
+                Cfg::OFF_OUT + ((from * (BN / 8 / SPLIT) + Cfg::chunk(i)) * 2 * kM + row) * 16);
             const uint32_t dst = cluster_addr(sbase + slot, to);
             st_cluster(dst, y[0], y[1], y[2], y[3]);
             st_cluster(dst + kM * 16, y[4], y[5], y[6], y[7]);
@@ -399,15 +401,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_ld8(acc + i * 8, own);
 #pragma unroll
                 for (int q = 0; q < SPLIT; ++q) {  // in order of K, whichever CTA adds
-                    const float4* part = reinterpret_cast<const float4*>(smem + Cfg::OFF_OUT) +
-                                         (q * (BN / 8 / SPLIT) + Cfg::chunk(i)) * 2 * kM + row;
-                    const float4 lo = part[0], hi = part[kM];
-                    const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                    float x[8];
+                    if (q == share) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float v = q == share ? own[e] : x[e];
-                        y[e] = q == 0 ? v : y[e] + v;
+                        for (int e = 0; e < 8; ++e) x[e] = own[e];
+                    } else {
+                        const int from = q < share ? q : q - 1;
+                        const float4* part =
+                            reinterpret_cast<const float4*>(smem + Cfg::OFF_OUT) +
+                            (from * (BN / 8 / SPLIT) + Cfg::chunk(i)) * 2 * kM + row;
+                        const float4 lo = part[0], hi = part[kM];
+                        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
+                        x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
                     }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = q == 0 ? x[e] : y[e] + x[e];
                 }
                 if (a.bias) {
                     const __half* b = a.bias + (GATED && i * 8 >= Cfg::ON ? a.n + col : col);
@@ -612,18 +620,24 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     };
     if (activation == ACT_SWIGLU) {
         for (int i = 2; i <= 8; i *= 2) offer(split_time(64, 128, 170, i), i);
+        offer(split_time(128, 256, 256, 2), 1);
     } else {
         for (int i = 2; i <= 8; i *= 2) offer(split_time(64, 64, 130, i), i);
         for (int i = 2; i <= 8; i *= 2) offer(split_time(128, 128, 170, i), 16 + i);
+        offer(split_time(192, 192, 210, 2), 0);
+        offer(split_time(256, 256, 256, 2), 1);
     }
     auto launch_split = [&]() {
         switch (activation == ACT_SWIGLU ? 32 + sp.which : sp.which) {
+            case 0: return launch<192, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
+            case 1: return launch<256, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
             case 2: return launch<64, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
             case 4: return launch<64, false, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
             case 8: return launch<64, false, false, 8>(x, ldx, w, ldw, out, ldo, a, s);
             case 18: return launch<128, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
             case 20: return launch<128, false, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
             case 24: return launch<128, false, false, 8>(x, ldx, w, ldw, out, ldo, a, s);
+            case 33: return launch<256, true, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
             case 34: return launch<128, true, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
             case 36: return launch<128, true, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
             default: return launch<128, true, false, 8>(x, ldx, w, ldw, out, ldo, a, s);

@@ -86,15 +86,17 @@ def _int32(t: torch.Tensor, numel: int | None, what: str) -> None:
         raise _lib.InvalidShape(f"{what} must have {numel} entries, got {t.numel()}")
 
 
-def _stride(t: torch.Tensor, heads: int, d: int, what: str) -> int:
+def _stride(t: torch.Tensor, rows: int, heads: int, d: int, what: str) -> int:
     """Row stride of a [rows, heads, D] tensor with packed heads (a view into a wider fused
     projection is fine); 0 (packed) for one row, whose stride means nothing."""
     shape, stride = t.shape, t.stride()
     if len(shape) != 3 or shape[1] != heads or shape[2] != d:
         raise _lib.ModelFormat(f"{what} must be [rows, {heads}, {d}], got {list(shape)}")
+    if shape[0] != rows:
+        raise _lib.ShapeMismatch(f"{what} must have {rows} rows", left=shape, right=[rows, heads, d])
     if stride[2] != 1 and d > 1 or stride[1] != d and heads > 1:
         raise _lib.NonContiguousTensor(f"{what} heads must be packed rows of {d} elements")
-    if shape[0] <= 1:
+    if rows <= 1:
         return 0
     if stride[0] < heads * d:  # rows over one another (an expanded tensor)
         raise _lib.NonContiguousTensor(f"{what} rows overlap: stride {stride[0]}")
@@ -170,24 +172,21 @@ def rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             q_out is not None and q_out.dtype != dtype) or (
             k_out is not None and k_out.dtype != dtype):
         raise _lib.UnsupportedDType("q, k, v and the cache must have one dtype")
-    qs, ks = _stride(q, hq, d, "q"), _stride(k, hkv, d, "k")
-    if _stride(v, hkv, d, "v") != ks:
+    qs, ks = _stride(q, rows, hq, d, "q"), _stride(k, rows, hkv, d, "k")
+    if _stride(v, rows, hkv, d, "v") != ks:
         raise _lib.NonContiguousTensor("k and v must have the same row stride")
-    if k.shape[0] != rows or v.shape[0] != rows:
-        raise _lib.ShapeMismatch("k and v must have q's rows", left=k.shape, right=v.shape)
     _int32(positions, rows, "positions")
     if slots.dtype != torch.int64 or slots.numel() != rows or not slots.is_contiguous():
         raise _lib.InvalidArgument("slots must be a contiguous int64 tensor of rows entries")
     if q_out is None:
-        q_out = torch.zeros((rows, hq, d), dtype=q.dtype, device=dev)
-    elif q_out.shape != q.shape:
-        raise _lib.ShapeMismatch("q_out must have q's shape", left=q_out.shape, right=q.shape)
-    if k_out is not None and k_out.shape != k.shape:
-        raise _lib.ShapeMismatch("k_out must have k's shape", left=k_out.shape, right=k.shape)
+        q_out = torch.zeros((rows, hq, d), dtype=dtype, device=dev)
+    qos = _stride(q_out, rows, hq, d, "q_out")
+    kos = _stride(k_out, rows, hkv, d, "k_out") if k_out is not None else 0
     if rope is not None:
         if cos.dtype != torch.float32 or sin.dtype != torch.float32:
             raise _lib.UnsupportedDType("RoPE requires F32 cos/sin tables")
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] * 2 != d or not (
+        shape = cos.shape
+        if len(shape) != 2 or shape != sin.shape or shape[1] * 2 != d or not (
                 cos.is_contiguous() and sin.is_contiguous()):
             raise _lib.InvalidShape("RoPE cos/sin tables must be contiguous [positions, D/2]")
     if rows == 0:
@@ -196,8 +195,7 @@ def rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
           hq, qs, ks, positions.data_ptr(), slots.data_ptr(),
           cos.data_ptr() if cos is not None else None, sin.data_ptr() if sin is not None else None,
           cos.shape[0] if cos is not None else 0, q_out.data_ptr(),
-          _stride(q_out, hq, d, "q_out"), k_out.data_ptr() if k_out is not None else None,
-          _stride(k_out, hkv, d, "k_out") if k_out is not None else 0)
+          qos, k_out.data_ptr() if k_out is not None else None, kos)
     return q_out, k_out
 
 
@@ -223,11 +221,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise _lib.UnsupportedDType(f"prompt attention dtype mismatch: {q.dtype}, {k.dtype}, "
                                     f"{v.dtype}")
-    qs, ks = _stride(q, hq, d, "q"), _stride(k, hkv, d, "k")
-    if _stride(v, hkv, d, "v") != ks:
+    qs, ks = _stride(q, rows, hq, d, "q"), _stride(k, rows, hkv, d, "k")
+    if _stride(v, rows, hkv, d, "v") != ks:
         raise _lib.NonContiguousTensor("k and v must have the same row stride")
-    if k.shape[0] != rows or v.shape[0] != rows:
-        raise _lib.ShapeMismatch("k and v must have q's rows", left=k.shape, right=v.shape)
     _int32(q_start, None, "q_start")
     if q_start.numel() < 2:
         raise _lib.InvalidShape("q_start must have num_seqs + 1 entries")
@@ -241,7 +237,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
                                    "F32")
     if lse is None and want_lse:
         lse = torch.zeros((rows, hq), dtype=torch.float32, device=dev)
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (rows, hq)
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, hq)
                             or not lse.is_contiguous()):
         raise _lib.InvalidArgument("lse must be a contiguous F32 [rows, Hq] tensor")
     _call(dev, "tmllm_prompt_attention", dt, q.data_ptr(), qs, k.data_ptr(), v.data_ptr(), ks,

@@ -534,7 +534,8 @@ def test_prompt_linear_pairs_of_ctas(cuda, rows, k, n):
     (33, 4096, 64, "none"), (1, 4104, 88, "gelu"), (130, 4096, 512, "relu"), (33, 4040, 1000, "silu"),
     (512, 1024, 1024, "none"), (256, 4096, 4096, "gelu"), (33, 4096, 4096, "none"),
     (33, 8192, 1016, "silu"), (33, 4096, 2048, "swiglu"), (9, 2048, 2560, "swiglu"),
-    (70, 4104, 488, "swiglu"), (129, 520, 40, "none")])
+    (70, 4104, 488, "swiglu"), (129, 520, 40, "none"), (300, 4096, 4088, "gelu"),
+    (500, 4104, 4096, "none"), (300, 4096, 2040, "swiglu")])
 def test_prompt_linear_long_products_of_few_tiles(cuda, rows, k, n, act):
     """K split over 2, 4 and 8 CTAs, columns and K that no part divides."""
     linear_case(cuda, rows, k, n, act, bias=True, residual=True, seed=rows, xpad=8, opad=8, wpad=16)
