@@ -605,6 +605,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + B::COUNT * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* odd_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);  // scrub found any
+    int* top_cost = reinterpret_cast<int*>(tmem_slot + 3);
     constexpr unsigned FULL = 0xffffffffu;
 
     if (tid == 0) {
@@ -615,6 +616,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         *abort_flag = 0;
         *odd_flag = 0;
+        *top_cost = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) {
@@ -659,18 +661,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!sorted) {
             for (int i = tid; i < count; i += kTcThreads) list[i] = static_cast<uint16_t>(ea + i);
         } else {
+            int top = 0;
             for (int i = tid; i < count; i += kTcThreads) {
                 const int t0 = max((ea + i) * span, ta), t1 = min((ea + i) * span + span, tb) - 1;
                 const int first = static_cast<int>(tile_first[t0] & ~AttSched::kSeveral);
                 const int c = tile0 + t1 - first / kTile;
                 cost[i] = static_cast<uint16_t>(c < kWindow ? c : kWindow - 1);
                 atomicAdd(hist + cost[i], 1);
+                top = max(top, static_cast<int>(cost[i]));
             }
+            __syncwarp();
+            top = __reduce_max_sync(FULL, top);
+            if (lane == 0 && top > 0) atomicMax(top_cost, top);
             __syncthreads();
             if (warp == 0) {
                 int above = 0;  // entries of a higher cost
-                const int most = tile0 + tb < kWindow ? tile0 + tb : kWindow - 1;
-                for (int c0 = most; c0 >= 0; c0 -= 32) {
+                for (int c0 = *top_cost; c0 >= 0; c0 -= 32) {
                     const int c = c0 - lane, own = c >= 0 ? hist[c] : 0;
                     int sum = own;
 #pragma unroll
