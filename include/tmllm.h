@@ -454,7 +454,8 @@ int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, co
  *   lse      [rows, q_heads] F32 natural-log sums of the scaled logits (NULL ok)
  * Keys and values behind a row do not reach its result, whatever they hold.  A row whose
  * logits are all -inf gives zeros and lse -inf.  F16 with head_dim a multiple of 8 up to 128
- * and 16-byte aligned rows runs on the tensor cores, everything else on the CUDA cores. */
+ * and 16-byte aligned rows runs on the tensor cores, everything else on the CUDA cores.  The order
+ * of a row's sums depends on rows and num_seqs, never on the run. */
 int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, const void* k,
                            const void* v, int64_t kv_stride, const int32_t* q_start,
                            int32_t num_seqs, int64_t rows, int32_t max_rows, int32_t q_heads,
@@ -468,7 +469,8 @@ int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, c
  *   4 swiglu: W is [k, 2n], gate then up columns, out = residual + silu(gate) * up;
  *   bias F16 [n] (swiglu [2n]) or NULL; residual F16 [rows, n] or NULL (may be out itself).
  * k and n multiples of 8, row strides multiples of 8 elements, x / W / residual / out 16-byte
- * aligned. */
+ * aligned.  The order of the sums over k depends on rows, k and n (few rows and a long k are split),
+ * never on the run. */
 int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                         int32_t activation, const void* residual, int64_t ldr, void* out,
                         int64_t ldo, int32_t rows, int32_t k, int32_t n, tmllm_stream stream);
