@@ -977,13 +977,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (ok) load_kv(&vmap, j);
                 }
             }
-            if (!ok) {  // another role gave up: let the copies in flight land
-                for (int i = ring < Cfg::STAGES ? 0 : ring - Cfg::STAGES; i < ring; ++i)
-                    mbar_drain(bar(B::KF + i % Cfg::STAGES), (i / Cfg::STAGES) & 1);
-                for (int i = 0; i < 2; ++i)
-                    for (int n = cnt[i] < Cfg::QBUF ? 0 : cnt[i] - Cfg::QBUF; n < cnt[i]; ++n)
-                        mbar_drain(bar(B::QF + (n % Cfg::QBUF) * 2 + i), (n / Cfg::QBUF) & 1);
-            }
+            // every copy has landed before the CTA gives its memory back, also when this warp got
+            // through and another one gave up
+            for (int i = ring < Cfg::STAGES ? 0 : ring - Cfg::STAGES; i < ring; ++i)
+                mbar_drain(bar(B::KF + i % Cfg::STAGES), (i / Cfg::STAGES) & 1);
+            for (int i = 0; i < 2; ++i)
+                for (int n = cnt[i] < Cfg::QBUF ? 0 : cnt[i] - Cfg::QBUF; n < cnt[i]; ++n)
+                    mbar_drain(bar(B::QF + (n % Cfg::QBUF) * 2 + i), (n / Cfg::QBUF) & 1);
         } else if (warp == 9 || warp == 10) {
             // One MMA warp an item: while one waits for its softmax group the other one's
             // products run.  The whole warp walks this code and one elected lane issues: with

@@ -81,7 +81,8 @@ struct LinCfg {
     static constexpr int STAGES = RING / STAGE < 8 ? RING / STAGE : 8;
     static constexpr int OFF_OUT = STAGES * STAGE;
     static constexpr int OFF_BIAS = OFF_OUT + OUT_BYTES;
-    static constexpr int OFF_BAR = OFF_BIAS + 2 * BN * 2;  // bias as F16
+    // bias as F16: 32 columns (and the 32 up columns of a gated tile) of each epilogue warp
+    static constexpr int OFF_BAR = OFF_BIAS + kEpiWarps * 64 * 2;
     static constexpr int SMEM = OFF_BAR + 512 + 1024;  // + alignment
     static constexpr int ACC = BN <= 64 ? 64 : BN <= 128 ? 128 : 256;  // columns apart
     static constexpr int TMEM_COLS = 2 * ACC;                          // two accumulators
@@ -206,7 +207,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            for (int i = g < Cfg::STAGES ? 0 : g - Cfg::STAGES; !ok && rank == 0 && i < g; ++i)
+            // every copy has landed before the CTA gives its memory back, also when this warp
+            // got through and another one gave up
+            for (int i = g < Cfg::STAGES ? 0 : g - Cfg::STAGES; rank == 0 && i < g; ++i)
                 mbar_drain(full(i % Cfg::STAGES), (i / Cfg::STAGES) & 1);
         }
     } else if (warp == 1 && rank == 0) {
@@ -276,38 +279,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp > 1) {
         // ---- epilogue: a warp owns 32 rows and every other 32 columns of the tile.  It works
         // alone: its rows leave through its own two buffers and bulk stores; the residual
-        // arrives the same way in the buffer it leaves by, 32 columns ahead.
+        // arrives the same way in the buffer it leaves by, 32 columns ahead, and the bias by a
+        // load a lane, 32 columns ahead too.  No barrier joins the warps: one that gave up a wait
+        // leaves by itself, and a barrier has no limit.
         const int quarter = warp & 3, part = (warp - 2) >> 2;
-        __half* bias_s = reinterpret_cast<__half*>(smem + Cfg::OFF_BIAS);
+        __half* bias = reinterpret_cast<__half*>(smem + Cfg::OFF_BIAS) + (warp - 2) * 64;
         unsigned char* stage = smem + Cfg::OFF_OUT + (warp - 2) * 4096;
         const uint32_t stage_addr = smem_u32(stage);
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
         int it = 0, ob = 0;
         uint32_t phases[2] = {0u, 0u};
+        uint32_t sent = 0;  // bit b: an odd number of residual loads went to buffer b
         for (int t = tile_first; t < a.tiles && !*abort_flag; t += tile_step, ++it) {
             int m, n;
             tile_of(a, t, m, n);
             const int ab = it & 1;
-            __half* bias = bias_s + ab * BN;
-            if (a.bias) {
-                for (int c = tid - 64; c < BN; c += 32 * kEpiWarps) {
-                    const int col = GATED ? n * Cfg::ON + c % Cfg::ON : n * BN + c;
-                    const bool in = col < a.n;
-                    bias[c] = in ? a.bias[GATED && c >= Cfg::ON ? a.n + col : col] : __half(0.f);
-                }
-                named_barrier(1, 32 * kEpiWarps);
-            }
+            __half bias_next[2] = {__half(0.f), __half(0.f)};  // this lane's of the next columns
+            auto load_bias = [&](int c0) {
+                const int col = n * Cfg::ON + c0 + lane;
+                if (!a.bias || c0 >= Cfg::ON || col >= a.n) return;
+                bias_next[0] = a.bias[col];
+                if (GATED) bias_next[1] = a.bias[a.n + col];
+            };
             // columns c0 .. of the tile into buffer b, once its last store has been read
             auto load_res = [&](int c0, int b) {
                 const int col = n * Cfg::ON + c0;
                 if (!a.residual || c0 >= Cfg::ON || col >= a.n || lane != 0) return;
                 bulk_wait_read<0>();
                 mbar_arrive_tx(res_full(warp - 2, b), 2048);
+                sent ^= 1u << b;
                 tma_load_2d(stage_addr + b * 2048, &rmap, col, row_of(m) + quarter * 32,
                             res_full(warp - 2, b));
             };
             load_res(part * 32, ob);
+            load_bias(part * 32);
             mbar_wait_uniform(acc_full(ab), (it >> 1) & 1, abort_addr, &g_linear_status);
             tc_fence_after();
             const uint32_t acc = tmem + ab * Cfg::ACC + lane_base;
@@ -315,18 +321,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c0 = part * 32; c0 < Cfg::ON; c0 += 64, ob ^= 1) {
                 const int col0 = n * Cfg::ON + c0;
                 if (col0 >= a.n) break;  // uniform: the rest of the tile is outside
+                if (a.bias) {
+                    bias[lane] = bias_next[0];
+                    if (GATED) bias[32 + lane] = bias_next[1];
+                    __syncwarp();
+                    load_bias(c0 + 64);
+                }
                 float y[32];
                 tmem_ld32(acc + c0, y);
                 if (a.bias) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] += __half2float(bias[c0 + i]);
+                    for (int i = 0; i < 32; ++i) y[i] += __half2float(bias[i]);
                 }
                 if (GATED) {
                     float u[32];
                     tmem_ld32(acc + Cfg::ON + c0, u);
                     if (a.bias) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) u[i] += __half2float(bias[Cfg::ON + c0 + i]);
+                        for (int i = 0; i < 32; ++i) u[i] += __half2float(bias[32 + i]);
                     }
 #pragma unroll
                     for (int i = 0; i < 32; ++i) y[i] = silu(y[i]) * u[i];
@@ -381,7 +393,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else mbar_arrive(acc_empty(ab));
             }
         }
-        if (lane == 0) bulk_wait<0>();
+        if (lane == 0) {
+            bulk_wait<0>();
+            // a residual tile that nobody waited for (a wait was given up) has landed, too
+            for (int b = 0; b < 2; ++b) mbar_drain(res_full(warp - 2, b), (sent >> b & 1u) ^ 1u);
+        }
         __syncwarp();
     }
     __syncwarp();
