@@ -98,6 +98,23 @@ struct ExchangeArgs {
         if (tmllm_e_ != cudaSuccess) return ::tmllm::cuda_fail(tmllm_e_, "kernel launch"); \
     } while (0)
 
+namespace tmllm {
+// Reads and clears a kernel's status word (a __device__ int) on the current device, once all work
+// launched there has ended: streams that the default one does not wait for are waited for, too.  Only
+// a word that was read is cleared.
+template <typename Symbol> int take_status(Symbol& word, int* out) {
+    int v = 0;
+    TMLLM_CUDA_TRY(cudaDeviceSynchronize());
+    TMLLM_CUDA_TRY(cudaMemcpyFromSymbol(&v, word, sizeof(int)));
+    if (v) {
+        const int zero = 0;
+        TMLLM_CUDA_TRY(cudaMemcpyToSymbol(word, &zero, sizeof(int)));
+    }
+    *out = v;
+    return TMLLM_OK;
+}
+}  // namespace tmllm
+
 // ---- device helpers -------------------------------------------------------------------
 
 namespace tmllm {

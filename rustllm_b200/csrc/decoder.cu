@@ -1325,11 +1325,7 @@ int tmllm_swiglu(tmllm_dtype dtype, const void* gate_up, void* out, size_t rows,
 int tmllm_linear_status(int32_t* status) {
     clear_error();
     if (!status) return fail(TMLLM_INVALID_ARGUMENT, "null status pointer");
-    int v = 0, zero = 0;
-    TMLLM_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_linear_status, sizeof(int)));
-    TMLLM_CUDA_TRY(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)));
-    *status = v;
-    return TMLLM_OK;
+    return take_status(g_linear_status, status);
 }
 
 size_t tmllm_linear_stats_bytes(int32_t n) {

@@ -1154,11 +1154,7 @@ int tmllm_gqa_prefill(const tmllm_paged_kv* kv, const void* q, const void* k_new
 int tmllm_prefill_status(int32_t* status) {
     clear_error();
     if (!status) return fail(TMLLM_INVALID_ARGUMENT, "null status pointer");
-    int v = 0, zero = 0;
-    TMLLM_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_prefill_status, sizeof(int)));
-    TMLLM_CUDA_TRY(cudaMemcpyToSymbol(g_prefill_status, &zero, sizeof(int)));
-    *status = v;
-    return TMLLM_OK;
+    return take_status(g_prefill_status, status);
 }
 
 }  // extern "C"

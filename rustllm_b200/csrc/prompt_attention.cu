@@ -1180,10 +1180,9 @@ extern "C" {
 int tmllm_prompt_status(int32_t* status) {
     clear_error();
     if (!status) return fail(TMLLM_INVALID_ARGUMENT, "null status pointer");
-    int linear = 0, attention = 0, zero = 0;
+    int linear = 0, attention = 0;
     if (int st = take_linear_wait_status(&linear)) return st;
-    TMLLM_CUDA_TRY(cudaMemcpyFromSymbol(&attention, g_attention_status, sizeof(int)));
-    TMLLM_CUDA_TRY(cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(int)));
+    if (int st = take_status(g_attention_status, &attention)) return st;
     *status = linear ? linear : attention;
     return TMLLM_OK;
 }

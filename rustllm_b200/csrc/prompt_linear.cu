@@ -548,13 +548,7 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, in
 
 }  // namespace
 
-int take_linear_wait_status(int* out) {
-    int v = 0, zero = 0;
-    TMLLM_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_linear_status, sizeof(int)));
-    TMLLM_CUDA_TRY(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)));
-    *out = v;
-    return TMLLM_OK;
-}
+int take_linear_wait_status(int* out) { return take_status(g_linear_status, out); }
 
 }  // namespace tmllm
 

@@ -25,3 +25,27 @@ def test_prompt_linear_many_tiles_a_cta(cuda, rows, n, act):
     linear_case(cuda, rows, 200, n, act, bias=True, residual=True, seed=rows)
     linear_case(cuda, rows, 200, n, act, bias=True, seed=rows + 1, xpad=8)
     linear_case(cuda, rows, 72, n, act, residual=True, inplace=True, seed=rows + 2)
+
+
+# ---- the status of the bounded waits ----------------------------------------------------
+@pytest.mark.parametrize("name", ["prompt_status", "prefill_status", "linear_status"])
+def test_status_waits_for_work_on_every_stream(cuda, name):
+    """A status is that of all work launched before it, on streams that the default stream does
+    not wait for, too."""
+    from rustllm_b200.decoder import linear_status
+    status = dict(prompt_status=rb.prompt_status, prefill_status=rb.prefill_status,
+                  linear_status=linear_status)[name]
+    g = gen(cuda, 1)
+    q, k = randn(g, 8192, 32, 128), randn(g, 8192, 8, 128)
+    starts = torch.tensor([0, 8192], dtype=torch.int32, device=cuda)
+    out = torch.zeros_like(q)
+    rb.prompt_attention(q, k, k, starts, 8192, out=out)
+    status()  # (the first read loads its kernels, which waits)
+    side, done = torch.cuda.Stream(cuda), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            rb.prompt_attention(q, k, k, starts, 8192, out=out)
+        done.record()
+    assert status() == 0
+    assert done.query()
