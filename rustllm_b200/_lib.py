@@ -116,7 +116,28 @@ _BY_STATUS = {cls.status: cls for cls in (
     DeviceTimeout, NotReserved)}
 
 
-class PagedKV(C.Structure):
+def as_i32(value: int, what: str) -> int:
+    """``value`` for a 32-bit field or parameter, of which ctypes would take the low bits."""
+    if not -0x80000000 <= value <= 0x7FFFFFFF:
+        raise InvalidShape(f"{what} must fit 32 bits, got {value}")
+    return value
+
+
+class _Checked(C.Structure):
+    """A structure whose 32-bit fields refuse values that do not fit (given by keyword)."""
+
+    def __init__(self, **fields):
+        narrow = self._narrow_
+        for name, value in fields.items():
+            if name in narrow:
+                as_i32(value, name)
+        super().__init__(**fields)
+
+    def __init_subclass__(cls):
+        cls._narrow_ = frozenset(name for name, kind in cls._fields_ if kind is i32)
+
+
+class PagedKV(_Checked):
     """``tmllm_paged_kv``: device pointers of one layer's block-paged store."""
 
     _fields_ = [("k_cache", vp), ("v_cache", vp), ("block_table", vp), ("seq_lens", vp),
@@ -125,7 +146,7 @@ class PagedKV(C.Structure):
                 ("dtype", i32)]
 
 
-class DecodeOpts(C.Structure):
+class DecodeOpts(_Checked):
     """``tmllm_decode_opts``."""
 
     _fields_ = [("scale", C.c_float), ("num_splits", i32), ("out_f32", i32),
@@ -134,7 +155,7 @@ class DecodeOpts(C.Structure):
                 ("flags", i32), ("q_seq_stride", i64), ("kv_seq_stride", i64)]
 
 
-class CacheConfig(C.Structure):
+class CacheConfig(_Checked):
     """``tmllm_cache_config``."""
 
     _fields_ = [("device", i32), ("num_layers", i32), ("num_seqs", i32),
@@ -227,6 +248,10 @@ _PROTOS = {
                                       vp]),
 }
 
+# where the 32-bit parameters of each function are
+_NARROW = {name: tuple(i for i, kind in enumerate(args) if kind is i32)
+           for name, (_, args) in _PROTOS.items()}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -280,4 +305,7 @@ def check(rc: int) -> None:
 
 
 def call(name: str, *args) -> None:
+    for i in _NARROW[name]:
+        if not -0x80000000 <= args[i] <= 0x7FFFFFFF:
+            as_i32(args[i], f"argument {i} of {name}")
     check(getattr(load(), name)(*args))

@@ -58,7 +58,8 @@ def gqa_decode(kv: PagedKV, q: torch.Tensor, k_new: torch.Tensor | None,
                       variant=variant)
     if rope is not None:
         cos, sin = rope
-        opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), \
+            _lib.as_i32(cos.shape[0], "RoPE table rows")
     call("tmllm_gqa_decode", C.byref(kv), q.data_ptr(),
          k_new.data_ptr() if k_new is not None else None,
          v_new.data_ptr() if v_new is not None else None, out.data_ptr(),
@@ -140,7 +141,8 @@ def gqa_prefill(kv: PagedKV, q: torch.Tensor, k_new: torch.Tensor | None,
                       kv_seq_stride=ks)
     if rope is not None:
         cos, sin = rope
-        opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), \
+            _lib.as_i32(cos.shape[0], "RoPE table rows")
     if q_start is not None:
         if q_start.dtype != torch.int32 or q_start.numel() != kv.num_seqs + 1:
             raise _lib.InvalidArgument("q_start must be int32 [num_seqs + 1]")

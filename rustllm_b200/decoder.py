@@ -415,7 +415,8 @@ class Decoder:
         opts = DecodeOpts(q_seq_stride=w, kv_seq_stride=w, max_len_hint=self.max_len_hint,
                           flags=DECODE_OVERLAP)
         cos, sin = self.rope
-        opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), \
+            _lib.as_i32(cos.shape[0], "RoPE table rows")
         call("tmllm_cache_decode", self.cache.handle, layer, base, base + hq * d * es,
              base + (hq + hkv) * d * es, self.attn.data_ptr(), None, hq, C.byref(opts),
              stream_ptr(self.device))

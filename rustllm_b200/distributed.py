@@ -211,7 +211,8 @@ class SequenceSplitAttention:
             o.max_len_hint = self._local_len + 1
             if rope is not None:
                 cos, sin = rope
-                o.rope_cos, o.rope_sin, o.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+                o.rope_cos, o.rope_sin, o.rope_len = cos.data_ptr(), sin.data_ptr(), \
+                    _lib.as_i32(cos.shape[0], "RoPE table rows")
             args = (C.byref(self._kv), key[0], key[1], key[2], key[3], None, self.hq,
                     C.byref(o), self.ws.ptr, self.ws.nbytes, self.peer.handle, key[-1])
             self._argc[key] = args

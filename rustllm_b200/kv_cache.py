@@ -191,7 +191,8 @@ class PagedKvCache:
                           flags=_lib.DECODE_OVERLAP if overlap else 0)
         if rope is not None:
             cos, sin = rope
-            opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+            opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), \
+                _lib.as_i32(cos.shape[0], "RoPE table rows")
         q = q.contiguous()
         kp = k_new.contiguous().data_ptr() if k_new is not None else None
         vp = v_new.contiguous().data_ptr() if v_new is not None else None
@@ -239,7 +240,8 @@ class PagedKvCache:
                           kv_seq_stride=ks)
         if rope is not None:
             cos, sin = rope
-            opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+            opts.rope_cos, opts.rope_sin, opts.rope_len = cos.data_ptr(), sin.data_ptr(), \
+                _lib.as_i32(cos.shape[0], "RoPE table rows")
         call("tmllm_cache_prefill", self._h, layer, q.data_ptr(), k_new.data_ptr(),
              v_new.data_ptr(), n, out.data_ptr(), hq, C.byref(opts), self._stream())
         return out

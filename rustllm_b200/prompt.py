@@ -103,6 +103,12 @@ def _stride(t: torch.Tensor, rows: int, heads: int, d: int, what: str) -> int:
     return stride[0]
 
 
+def _wide(what: str):
+    """The refusal of sizes that the C call takes in 32 bits: ctypes would take the low bits of
+    larger ones.  (The callers test several sizes at once, or-ed together.)"""
+    return _lib.InvalidShape(f"{what} must fit 31 bits")
+
+
 def batch_tables(kv: PagedKV, new_lens: torch.Tensor, rows: int, *,
                  free_blocks: torch.Tensor | None = None,
                  free_start: torch.Tensor | None = None,
@@ -121,6 +127,9 @@ def batch_tables(kv: PagedKV, new_lens: torch.Tensor, rows: int, *,
     _int32(new_lens, n, "new_lens")
     if free_blocks is not None:
         _int32(free_blocks, None, "free_blocks")
+        num_free = free_blocks.numel()
+        if num_free >> 31:
+            raise _wide("the number of free blocks")
     if free_start is not None:
         if free_blocks is None:
             raise _lib.InvalidArgument("free_start needs free_blocks")
@@ -140,7 +149,7 @@ def batch_tables(kv: PagedKV, new_lens: torch.Tensor, rows: int, *,
     # an empty free list is not "no list": any non-null pointer stands for it (never read)
     _call(dev, "tmllm_batch_tables", C.byref(kv), new_lens.data_ptr(),
           (free_blocks.data_ptr() or new_lens.data_ptr()) if free_blocks is not None else None,
-          free_blocks.numel() if free_blocks is not None else 0,
+          num_free if free_blocks is not None else 0,
           free_start.data_ptr() if free_start is not None else None, rows,
           out.q_start.data_ptr(), out.positions.data_ptr(), out.row_seq.data_ptr(),
           out.slots.data_ptr(), out.info.data_ptr())
@@ -165,6 +174,8 @@ def rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise _lib.ModelFormat(f"q must be [rows, Hq, D], got {list(q.shape)}")
     rows, hq, d = q.shape
     hkv = kv.num_kv_heads
+    if hq >> 31:
+        raise _wide("the number of heads")
     if d != kv.head_dim:
         raise _lib.ModelFormat(f"the cache holds heads of {kv.head_dim}, got {d}")
     dtype = q.dtype
@@ -189,12 +200,15 @@ def rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         if len(shape) != 2 or shape != sin.shape or shape[1] * 2 != d or not (
                 cos.is_contiguous() and sin.is_contiguous()):
             raise _lib.InvalidShape("RoPE cos/sin tables must be contiguous [positions, D/2]")
+        rope_len = shape[0]
+        if rope_len >> 31:
+            raise _wide("the rows of the RoPE tables")
     if rows == 0:
         return q_out, k_out
     _call(dev, "tmllm_rope_append", C.byref(kv), q.data_ptr(), k.data_ptr(), v.data_ptr(), rows,
           hq, qs, ks, positions.data_ptr(), slots.data_ptr(),
           cos.data_ptr() if cos is not None else None, sin.data_ptr() if sin is not None else None,
-          cos.shape[0] if cos is not None else 0, q_out.data_ptr(),
+          rope_len if cos is not None else 0, q_out.data_ptr(),
           qos, k_out.data_ptr() if k_out is not None else None, kos)
     return q_out, k_out
 
@@ -227,6 +241,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
     _int32(q_start, None, "q_start")
     if q_start.numel() < 2:
         raise _lib.InvalidShape("q_start must have num_seqs + 1 entries")
+    if (q_start.numel() | hq | hkv | d | rows) >> 31:
+        raise _wide("the numbers of sequences, heads and rows")
     if max_rows < 0:
         raise _lib.InvalidShape(f"max_rows must not be negative, got {max_rows}")
     if out is None:
@@ -269,6 +285,8 @@ def prompt_linear(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None
     if act == 4 and wide % 2:
         raise _lib.InvalidShape(f"swiglu needs gate and up columns, got {wide}")
     n = wide // 2 if act == 4 else wide
+    if (rows | k | wide) >> 31:
+        raise _wide("rows and columns")
     if x.dtype != torch.float16:
         raise _lib.UnsupportedDType(f"prompt_linear takes F16 tensors, got {x.dtype}")
     for t, what in ((w, "w"), (bias, "bias"), (residual, "residual"), (out, "out")):

@@ -49,3 +49,13 @@ def test_status_waits_for_work_on_every_stream(cuda, name):
         done.record()
     assert status() == 0
     assert done.query()
+
+
+# ---- sizes past 32 bits -----------------------------------------------------------------
+def test_prompt_linear_refuses_rows_past_32_bits(cuda):
+    """2^32 rows are not 0 rows (the rows lie over one another: nothing may reach the GPU)."""
+    x = torch.ones(1, 8, dtype=torch.float16, device=cuda)
+    out = torch.zeros(1, 8, dtype=torch.float16, device=cuda)
+    with pytest.raises(rb.InvalidShape):
+        rb.prompt_linear(x.expand(2 ** 32, 8), torch.ones(8, 8, dtype=torch.float16, device=cuda),
+                         out=out.expand(2 ** 32, 8))

@@ -6,7 +6,9 @@ import re
 
 import pytest
 
+import rustllm_b200 as rb
 from conftest import ROOT
+from rustllm_b200 import _lib
 
 
 def source(name: str) -> str:
@@ -26,3 +28,37 @@ def test_roles_of_a_cta_meet_at_no_barrier_without_a_limit(name, first, last):
     meets = re.findall(r"named_barrier|__syncthreads|bar\.sync|barrier\.cta|cluster_sync_all",
                        text[lo:hi])
     assert meets == (["__syncthreads"] if last == "tcgen05.dealloc" else [])
+
+
+# ---- sizes past 32 bits -----------------------------------------------------------------
+BIG = 2 ** 32  # 0 in its low 32 bits
+
+
+@pytest.mark.parametrize("rows,k,n", [(BIG, 64, 128), (4, BIG + 64, 128), (4, 64, BIG + 128),
+                                      (4, -BIG + 64, 128)])
+def test_sizes_past_32_bits_are_refused_not_cut(rows, k, n):
+    p = 1 << 20
+    with pytest.raises(rb.InvalidShape):
+        _lib.call("tmllm_prompt_linear", p, 64, 2 * p, 128, None, 0, None, 0, 3 * p, 128, rows, k, n,
+                  None)
+
+
+def test_older_calls_refuse_sizes_past_32_bits():
+    with pytest.raises(rb.InvalidShape):
+        _lib.call("tmllm_merge_lse", 16, 16, BIG, 1, 8, 8, 1, 16, 0, None, None)
+    with pytest.raises(rb.InvalidShape):
+        _lib.call("tmllm_cache_reserve", None, BIG, 1, None)
+
+
+@pytest.mark.parametrize("make", [
+    lambda: _lib.PagedKV(num_seqs=BIG + 1), lambda: _lib.PagedKV(num_blocks=BIG, block_size=BIG + 16),
+    lambda: _lib.DecodeOpts(rope_len=BIG + 5), lambda: _lib.CacheConfig(max_seq_len=BIG + 64)])
+def test_descriptor_fields_past_32_bits_are_refused(make):
+    with pytest.raises(rb.InvalidShape):
+        make()
+
+
+def test_descriptors_keep_what_fits():
+    kv = _lib.PagedKV(num_blocks=2 ** 40, num_seqs=2 ** 31 - 1, dtype=-1)
+    assert (kv.num_blocks, kv.num_seqs, kv.dtype) == (2 ** 40, 2 ** 31 - 1, -1)
+    assert _lib.DecodeOpts(max_len_hint=2 ** 40, rope_pos_offset=-3).rope_pos_offset == -3
