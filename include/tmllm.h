@@ -452,8 +452,10 @@ int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, co
  *   out      [rows, q_heads, head_dim] packed (dtype, or F32 if out_f32); may be q itself
  *     (same type and stride), and must not overlap k or v
  *   lse      [rows, q_heads] F32 natural-log sums of the scaled logits (NULL ok)
- * Keys and values behind a row do not reach its result, whatever they hold.  A row whose
- * logits are all -inf gives zeros and lse -inf.  F16 with head_dim a multiple of 8 up to 128
+ * Keys and values behind a row do not reach its result, whatever they hold.  A value that is
+ * not finite makes its element of every row that sees it non-finite: as itself, or as NaN (0 * inf)
+ * where its weight rounds to zero.  A row whose logits are all -inf gives zeros and lse -inf, over
+ * any values.  F16 with head_dim a multiple of 8 up to 128
  * and 16-byte aligned rows runs on the tensor cores, everything else on the CUDA cores.  The order
  * of a row's sums depends on rows and num_seqs, never on the run. */
 int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, const void* k,

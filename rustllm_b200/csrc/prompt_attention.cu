@@ -306,11 +306,22 @@ __global__ void __launch_bounds__(TT * TEAMS) prompt_fma_kernel(const PromptArgs
             }
         }
     }
+    bool none = false;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) none |= l[i] == 0.f;
+    if (none) {  // every score of a row -inf: zeros, whatever the values are (0 * inf is not 0)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            if (l[i] != 0.f) continue;
+#pragma unroll
+            for (int c = 0; c < 2 * CG; ++c) o[i][c] = make_float2(0.f, 0.f);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         const int r = q_lo + RT * ty + i;
         if (r >= n) continue;
-        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];  // every score -inf: zeros
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
         const int64_t off = (row0 + r) * a.out_stride + static_cast<int64_t>(h) * D;
 #pragma unroll
         for (int c = 0; c < CG; ++c)
@@ -406,7 +417,8 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 // the maximum, and since 0 * inf is not 0, the non-finite entries of every V tile that some row
 // of the unit does not see whole are zeroed in shared memory before the product and added
 // afterwards to the rows that see them ("scrubbed" tiles: the diagonal, the tile where the
-// sequence starts, all tiles of an item whose rows belong to several sequences).
+// sequence starts, all tiles of an item whose rows belong to several sequences).  The mask of the
+// units that had some leaves out keys of no sequence, so that NaN in padding costs nothing.
 constexpr int kTile = 128;
 constexpr int kTcThreads = 384;
 constexpr int kWindow = 1024;    // row tiles a launch schedules (131,072 packed rows)
@@ -587,6 +599,40 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 }
 __device__ __forceinline__ bool odd_half(uint32_t bits) { return (bits & 0x7C00u) == 0x7C00u; }
 
+// What a stored row lacks (rare, and out of line: the mere code of it cost instruction fetches in
+// the hot loop; 512 prompts of 300 tokens, 9/3 heads of 64: 290 us inline, 272 without).  The
+// non-finite values that the scrub took out of V (`vg`: column 0 of the KV head) are added to a row
+// that sees keys first .. row.  A row without a key (`none`: every score -inf) becomes zeros, since
+// the product made NaN of 0 * inf in the tiles that were not scrubbed.
+__device__ __noinline__ void finish_row(const __half* vg, int64_t kv_stride, void* out, int out_f32,
+                                        int head_dim, int first, int row, bool any_several,
+                                        int tile0, int tile1, int unit_first, bool none) {
+    if (none) {
+        for (int i = 0; i < head_dim; ++i) {
+            if (out_f32) static_cast<float*>(out)[i] = 0.f;
+            else static_cast<__half*>(out)[i] = __half(0.f);
+        }
+        return;
+    }
+    for (int key = first; key <= row; ++key) {
+        const int t = key / 128;
+        if (!(any_several || t == tile0 || t == tile1 || t * 128 < unit_first)) {
+            key |= 127;  // a tile that was not scrubbed: to its end
+            continue;
+        }
+        for (int i = 0; i < head_dim; ++i) {
+            const __half hv = vg[key * kv_stride + i];
+            if (!odd_half(__half_as_ushort(hv))) continue;
+            if (out_f32) {
+                static_cast<float*>(out)[i] += __half2float(hv);
+            } else {
+                __half* o = static_cast<__half*>(out) + i;
+                *o = __float2half(__half2float(*o) + __half2float(hv));
+            }
+        }
+    }
+}
+
 template <int DP, int KS>
 __global__ void __launch_bounds__(kTcThreads, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap qmap,
@@ -604,7 +650,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     auto bar = [&](int i) { return bars + 8u * static_cast<uint32_t>(i); };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + B::COUNT * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* odd_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);  // scrub found any
+    // bit k % 32: the scrub took visible values out of the tiles of this CTA's unit k
+    volatile uint32_t* odd_units = tmem_slot + 2;
     int* top_cost = reinterpret_cast<int*>(tmem_slot + 3);
     constexpr unsigned FULL = 0xffffffffu;
 
@@ -615,7 +662,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(bar(i), group ? 128u : both ? 2u : 1u);
         }
         *abort_flag = 0;
-        *odd_flag = 0;
+        *odd_units = 0;
         *top_cost = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -751,6 +798,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         while (more && !*abort_flag) {
             x = y;
             const AttUnit now = u;
+            const uint32_t unit_bit = 1u << ((sched.k - 1) & 31);
             const int lo = x.lo, hi = x.hi, row = x.row, first = x.first, head = x.head;
             const bool live = x.live;
             float m = -INFINITY, l = 0.f;
@@ -858,7 +906,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ---- epilogue
             await(B::O + w, step - 1);
             tc_fence_after();
-            const float inv = l == 0.f ? 0.f : 1.f / l;  // every score -inf: zeros
+            const bool none = l == 0.f;  // every score -inf
+            const float inv = none ? 0.f : 1.f / l;
             const int64_t orow = (live ? row : 0) * a.out_stride +
                                  static_cast<int64_t>(head) * a.head_dim;
 #pragma unroll 1
@@ -910,36 +959,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (a.lse && live)
                 a.lse[static_cast<int64_t>(row) * a.q_heads + head] =
                     ((m == -INFINITY ? 0.f : m) + __log2f(l)) * kLn2;
-        }
-        // ---- the non-finite values that the scrub took out, added to the stored rows that see
-        // them: all units once more, here and not in the epilogue, where the mere code of this
-        // rare case cost instruction fetches (512 prompts of 300 tokens, 9/3 heads of 64: 290 us,
-        // 272 with it here)
-        __syncwarp();  // rows are stored by whichever lanes
-        if (__any_sync(FULL, *odd_flag != 0)) {
-            sched.k = 0;
-            while (next()) {
-                if (!y.live) continue;
-                const __half* vg = static_cast<const __half*>(a.v) +
-                                   static_cast<int64_t>(u.kvh) * a.head_dim;
-                const int64_t orow = y.row * a.out_stride +
-                                     static_cast<int64_t>(y.head) * a.head_dim;
-                for (int key = y.first; key <= y.row; ++key) {
-                    if (!u.ragged(key / kTile)) {
-                        key |= kTile - 1;  // to the tile's end
-                        continue;
-                    }
-                    for (int i = 0; i < a.head_dim; ++i) {
-                        const __half hv = vg[key * a.kv_stride + i];
-                        if (!odd_half(__half_as_ushort(hv))) continue;
-                        if (a.out_f32) {
-                            static_cast<float*>(a.out)[orow + i] += __half2float(hv);
-                        } else {
-                            __half* o = static_cast<__half*>(a.out) + orow + i;
-                            *o = __float2half(__half2float(*o) + __half2float(hv));
-                        }
-                    }
-                }
+            if (__any_sync(FULL, live && (none || (*odd_units & unit_bit)))) {
+                // (rows were stored by any lane: the vote and the barriers before it order that)
+                if (live)
+                    finish_row(static_cast<const __half*>(a.v) +
+                                   static_cast<int64_t>(now.kvh) * a.head_dim,
+                               a.kv_stride,
+                               static_cast<unsigned char*>(a.out) + orow * (a.out_f32 ? 4 : 2),
+                               a.out_f32, a.head_dim, first, row, now.any_several, now.tile[0],
+                               now.tile[1], now.first, none);
+                __syncwarp();
             }
         }
     } else {
@@ -1080,8 +1109,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         } else if (warp == 11) {
             // ---- scrub: a V tile that some row of the unit does not see whole loses its
-            // non-finite entries (and the flag says that some were found) before the products
-            // read it, while the softmax groups are at its scores
+            // non-finite entries (and the unit's bit says that a sequence's key had some) before
+            // the products read it, while the softmax groups are at its scores
             const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
             int x = 1;  // ring index of the V tile
             while (sched.template next<Cfg::KS>(a, u) && !*abort_flag) {
@@ -1106,12 +1135,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const __half2 sum = __hadd2(__hadd2(probe[0], probe[1]),
                                                     __hadd2(probe[2], probe[3]));
                         if (!(__low2float(sum) == 0.f && __high2float(sum) == 0.f)) {
-                            *odd_flag = 1;
+                            bool any = false;
                             for (int c = 0; c < Cfg::TILE / 512; ++c) {
                                 uint16_t* b = reinterpret_cast<uint16_t*>(v + 512 * c);
-                                for (int e = 0; e < 8; ++e)
-                                    if (odd_half(b[e])) b[e] = 0;
+                                // 16 bytes a lane of rows of 128, 128 rows a block of columns
+                                const int key = j * kTile + (lane / 8 + 4 * c) % kTile;
+                                for (int e = 0; e < 8; ++e) {
+                                    if (!odd_half(b[e])) continue;
+                                    b[e] = 0;
+                                    any |= key >= sched.row_lo && key < sched.row_hi;
+                                }
                             }
+                            if (any)
+                                atomicOr(const_cast<uint32_t*>(odd_units),
+                                         1u << ((sched.k - 1) & 31));
                             fence_async_smem();
                         }
                     }

@@ -59,3 +59,47 @@ def test_prompt_linear_refuses_rows_past_32_bits(cuda):
     with pytest.raises(rb.InvalidShape):
         rb.prompt_linear(x.expand(2 ** 32, 8), torch.ones(8, 8, dtype=torch.float16, device=cuda),
                          out=out.expand(2 ** 32, 8))
+
+
+# ---- prompt_attention: values that are not finite ---------------------------------------
+@pytest.mark.parametrize("dtype,d,out_dtype", [
+    (torch.float16, 64, None), (torch.float16, 128, None), (torch.float16, 80, torch.float32),
+    (torch.float16, 20, None), (torch.float32, 64, None), (torch.float32, 200, None)])
+@pytest.mark.parametrize("hq,hkv,pad", [(2, 1, 0), (3, 1, 700), (24, 8, 0)])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_prompt_attention_rows_without_a_key_are_zero(cuda, dtype, d, out_dtype, hq, hkv, pad, bad):
+    """Every logit -inf gives zeros and lse -inf, also over values that are not finite, in the tiles
+    that a row sees whole and in the others; in a row with a finite logit such a value shows."""
+    g = gen(cuda, d + hq)
+    dark, lens = 200, [70, 300, 40]
+    rows, a = sum(lens) + pad, lens[0]
+    q, k, v = randn(g, rows, hq, d, dtype=dtype).abs(), randn(g, rows, hkv, d, dtype=dtype), \
+        randn(g, rows, hkv, d, dtype=dtype)
+    k[a:a + dark] = -math.inf
+    v[a + 3, :, 1], v[a + 150, :, 2], v[a + 250, :, 3] = bad, bad, bad
+    clean = v.clone()
+    clean[[a + 3, a + 150, a + 250]] = 0
+    starts = torch.tensor([0, 70, 370, 410], dtype=torch.int32, device=cuda)
+    out, lse = rb.prompt_attention(q, k, v, starts, 300, out_dtype=out_dtype, want_lse=True)
+    want = rb.prompt_attention(q, k, clean, starts, 300, out_dtype=out_dtype)
+    torch.cuda.synchronize()
+    assert rb.prompt_status() == 0
+    # a query element that was drawn as 0 makes its row's logits 0 * inf = NaN, not -inf
+    none = torch.zeros(rows, hq, dtype=torch.bool, device=cuda)
+    none[a:a + dark] = True
+    odd = (q == 0).any(-1)
+    odd[:a], odd[a + 300:] = False, False
+    assert int(odd.sum()) < 9
+    assert bool((out[none & ~odd] == 0).all()) and bool((lse[none & ~odd] == -math.inf).all())
+    assert bool(torch.isnan(out[odd]).all()) and bool(torch.isnan(lse[odd]).all())
+    sees = ~none & ~odd
+    assert bool(torch.isfinite(lse[:sum(lens)][sees[:sum(lens)]]).all())
+    sees[:a + dark], sees[a + 300:] = False, False
+    assert not bool(torch.isfinite(out[sees][:, 1:3]).any())  # weight 0, not finite
+    sees[:a + 250] = False
+    shows = out[sees][:, 3]
+    assert bool((torch.isnan(shows) if math.isnan(bad) else shows == bad).all())
+    keep = ~odd[:, :, None].expand_as(out).clone()
+    keep[a + dark:a + 300, :, 1:3] = False
+    keep[a + 250:a + 300] = False  # the zeroed row of `clean` carries weight there
+    assert torch.equal(out[keep], want[keep])
