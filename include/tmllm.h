@@ -447,7 +447,8 @@ int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, co
  *     (0 = packed); head_dim <= 256
  *   q_start  device int32 [num_seqs + 1], non-decreasing first rows; sequences may be empty;
  *     rows in front of q_start[0] and from q_start[num_seqs] on are neither read nor written
- *   max_rows the longest sequence, or more (a bound for the launch)
+ *   max_rows the longest sequence, or about that: it sizes the launch, and results do not depend
+ *     on it (a captured call may meet longer sequences); 0: nothing is done
  *   scale    <= 0 means 1/sqrt(head_dim)
  *   out      [rows, q_heads, head_dim] packed (dtype, or F32 if out_f32); may be q itself
  *     (same type and stride), and must not overlap k or v

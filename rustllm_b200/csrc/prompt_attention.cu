@@ -42,12 +42,12 @@ __device__ __forceinline__ int seq_rows(const PromptArgs& a, int s, int64_t* row
     if (hi > a.rows) hi = a.rows;
     if (lo < 0 || lo >= hi) return 0;
     *row0 = lo;
-    const int64_t n = hi - lo;
-    return static_cast<int>(n < a.max_rows ? n : a.max_rows);
+    return static_cast<int>(hi - lo);
 }
 
 // ---- CUDA-core form: any type and head size up to 256 -----------------------------------
-// One CTA per (TT / 16 RT query rows, query head, sequence), TEAMS teams of TT threads that take
+// One CTA per (TT / 16 RT query rows, query head, sequence), which goes on to the rows a launch's
+// worth behind them in a sequence longer than the launch was sized for; TEAMS teams of TT threads that take
 // every TEAMS-th tile of keys each and are joined at the end.  Thread (ty, tx) of a team holds RT
 // rows from RT ty on of S (columns tx + 16 c of a tile of 64 keys) and of O (columns 4 tx + 64 c
 // on).  DP: head size rounded up to 64 / 128 / 256.  Both products run on packed F32 pairs (two
@@ -87,25 +87,17 @@ __device__ __forceinline__ bool barrier_or(int id, bool x) {
     return any != 0;
 }
 
+// Rows q_lo .. of query head h of the sequence of n rows from row0 on.
 template <typename T, int DP, int RT, int TT, int TEAMS>
-__global__ void __launch_bounds__(TT * TEAMS) prompt_fma_kernel(const PromptArgs a, int row_tiles,
-                                                                 int async) {
+__device__ __forceinline__ void fma_rows(const PromptArgs& a, float* fsm, int h, int64_t row0, int n,
+                                         int q_lo, int async) {
     using Cfg = FmaCfg<DP, RT, TT, TEAMS>;
     constexpr int ROWS = Cfg::ROWS, LD = Cfg::LD, LP = Cfg::LP, CG = DP / 64;
-    extern __shared__ __align__(16) float fsm[];
     float* qs = fsm;                          // [ROWS][LD]
     const int team = TEAMS == 1 ? 0 : threadIdx.x / TT;
     float* kv0 = qs + ROWS * LD + team * (Cfg::BUFS * Cfg::KV + Cfg::PS);  // [BUFS]: K [64][LD],
                                                                            // V [64][DP]
     float* ps = kv0 + Cfg::BUFS * Cfg::KV;                                 // [ROWS][LP]
-    const int64_t hb = static_cast<int64_t>(a.q_heads) * a.num_seqs;
-    const int tile = row_tiles - 1 - static_cast<int>(blockIdx.x / hb);
-    const int h = static_cast<int>(blockIdx.x % hb) % a.q_heads;
-    const int s = static_cast<int>(blockIdx.x % hb) / a.q_heads;
-    int64_t row0 = 0;
-    const int n = seq_rows(a, s, &row0);
-    const int q_lo = tile * ROWS;
-    if (q_lo >= n) return;
     const int kvh = h / a.group, D = a.head_dim;
     const int tid = threadIdx.x % TT, tx = tid & 15, ty = tid >> 4;
     const T* qg = static_cast<const T*>(a.q) + (row0 + q_lo) * a.q_stride +
@@ -337,6 +329,45 @@ __global__ void __launch_bounds__(TT * TEAMS) prompt_fma_kernel(const PromptArgs
         if (a.lse && tx == 0)
             a.lse[(row0 + r) * a.q_heads + h] =
                 ((m[i] == -INFINITY ? 0.f : m[i]) + log2f(l[i])) * kLn2;
+    }
+}
+
+// The same out of line, for the rows past the launch's.  One team of up to 128 columns: as a loop
+// around the code above the usual single pass was slower (F32, 64 x 700 tokens, 9/3 heads of 64:
+// 1115 us against 1081; 4096 tokens, 8/2 heads of 128: 934 against 928); the others are better off
+// with the loop (prompts of 50, 3 and 100 tokens, 9/3 heads of 64: 8.6 us against 9.8; 4 x 1000,
+// 8/2 heads of 256: 472 against 475).
+template <typename T, int DP, int RT, int TT, int TEAMS>
+__device__ __noinline__ void fma_more_rows(const PromptArgs& a, float* fsm, int h, int64_t row0,
+                                           int n, int q_lo, int async) {
+    __syncthreads();  // the rows before are done with the shared memory
+    fma_rows<T, DP, RT, TT, TEAMS>(a, fsm, h, row0, n, q_lo, async);
+}
+
+template <typename T, int DP, int RT, int TT, int TEAMS>
+__global__ void __launch_bounds__(TT * TEAMS) prompt_fma_kernel(const __grid_constant__ PromptArgs a,
+                                                                 int row_tiles, int async) {
+    constexpr int ROWS = FmaCfg<DP, RT, TT, TEAMS>::ROWS;
+    extern __shared__ __align__(16) float fsm[];
+    const int64_t hb = static_cast<int64_t>(a.q_heads) * a.num_seqs;
+    const int tile = row_tiles - 1 - static_cast<int>(blockIdx.x / hb);
+    const int h = static_cast<int>(blockIdx.x % hb) % a.q_heads;
+    const int s = static_cast<int>(blockIdx.x % hb) / a.q_heads;
+    int64_t row0 = 0;
+    const int n = seq_rows(a, s, &row0);
+    const int64_t step = static_cast<int64_t>(row_tiles) * ROWS;
+    int64_t q_lo = static_cast<int64_t>(tile) * ROWS;
+    if constexpr (TEAMS == 1 && DP <= 128) {
+        if (q_lo >= n) return;
+        fma_rows<T, DP, RT, TT, TEAMS>(a, fsm, h, row0, n, static_cast<int>(q_lo), async);
+        for (q_lo += step; q_lo < n; q_lo += step)
+            fma_more_rows<T, DP, RT, TT, TEAMS>(a, fsm, h, row0, n, static_cast<int>(q_lo), async);
+    } else {
+        while (q_lo < n) {
+            fma_rows<T, DP, RT, TT, TEAMS>(a, fsm, h, row0, n, static_cast<int>(q_lo), async);
+            q_lo += step;
+            if (q_lo < n) __syncthreads();  // the rows are done with the shared memory
+        }
     }
 }
 

@@ -103,3 +103,37 @@ def test_prompt_attention_rows_without_a_key_are_zero(cuda, dtype, d, out_dtype,
     keep[a + dark:a + 300, :, 1:3] = False
     keep[a + 250:a + 300] = False  # the zeroed row of `clean` carries weight there
     assert torch.equal(out[keep], want[keep])
+
+
+# ---- prompt_attention: sequences longer than the launch bound ---------------------------
+@pytest.mark.parametrize("dtype,d", [(torch.float16, 64), (torch.float16, 128), (torch.float16, 136),
+                                     (torch.float16, 20), (torch.float32, 64), (torch.float32, 128),
+                                     (torch.float32, 256)])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (48, 4)])
+def test_prompt_attention_longer_than_max_rows(cuda, dtype, d, hq, hkv):
+    """max_rows sizes the launch: rows past it are computed all the same (a captured call meets
+    longer prompts than it was captured with)."""
+    for bound in (1, 70, 130):
+        attention_case(cuda, [5, 300, 0, 131, 64], hq, hkv, d, dtype, seed=d, pad=3, lead=2,
+                       max_rows=bound)
+    attention_case(cuda, [200, 330], hq, hkv, d, dtype, seed=d, max_rows=1, inplace=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_prompt_attention_captured_for_shorter_prompts(cuda, dtype):
+    g = gen(cuda, 4)
+    q, k, v = (randn(g, 400, h, 64, dtype=dtype) for h in (4, 2, 2))
+    starts = torch.tensor([0, 40, 400], dtype=torch.int32, device=cuda)
+    want = rb.prompt_attention(q, k, v, starts, 360)
+    live = torch.tensor([0, 200, 400], dtype=torch.int32, device=cuda)
+    out = torch.zeros_like(q)
+    rb.prompt_attention(q, k, v, live, 200, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rb.prompt_attention(q, k, v, live, 200, out=out)
+    live.copy_(starts)
+    out.fill_(7)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
