@@ -171,12 +171,17 @@ def prefill_status() -> int:
 def paged_kv_from_tensors(k_arena: torch.Tensor, v_arena: torch.Tensor,
                           block_table: torch.Tensor, seq_lens: torch.Tensor) -> PagedKV:
     """A ``PagedKV`` over caller-owned tensors: arenas [num_blocks, Hkv, block_size, D],
-    block_table int32 [num_seqs, max_blocks], seq_lens int32 [num_seqs]."""
+    block_table int32 [num_seqs, max_blocks], seq_lens int32 [num_seqs].  They live as long as
+    it does."""
     if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise _lib.UnsupportedDType("block table and lengths must be int32")
     nb, hkv, bs, d = k_arena.shape
-    return PagedKV(k_cache=k_arena.data_ptr(), v_cache=v_arena.data_ptr(),
-                   block_table=block_table.data_ptr(), seq_lens=seq_lens.data_ptr(),
-                   num_blocks=nb, num_seqs=block_table.shape[0], num_kv_heads=hkv, head_dim=d,
-                   block_size=bs, max_blocks_per_seq=block_table.shape[1],
-                   dtype=dtype_code(k_arena.dtype))
+    kv = PagedKV(k_cache=k_arena.data_ptr(), v_cache=v_arena.data_ptr(),
+                 block_table=block_table.data_ptr(), seq_lens=seq_lens.data_ptr(),
+                 num_blocks=nb, num_seqs=block_table.shape[0], num_kv_heads=hkv, head_dim=d,
+                 block_size=bs, max_blocks_per_seq=block_table.shape[1],
+                 dtype=dtype_code(k_arena.dtype))
+    # the descriptor keeps its tensors: over a temporary it would point at memory that the
+    # allocator gives to the next one
+    kv.tensors = (k_arena, v_arena, block_table, seq_lens)
+    return kv

@@ -5,6 +5,7 @@ import os
 import re
 
 import pytest
+import torch
 
 import rustllm_b200 as rb
 from conftest import ROOT
@@ -62,3 +63,20 @@ def test_descriptors_keep_what_fits():
     kv = _lib.PagedKV(num_blocks=2 ** 40, num_seqs=2 ** 31 - 1, dtype=-1)
     assert (kv.num_blocks, kv.num_seqs, kv.dtype) == (2 ** 40, 2 ** 31 - 1, -1)
     assert _lib.DecodeOpts(max_len_hint=2 ** 40, rope_pos_offset=-3).rope_pos_offset == -3
+
+
+# ---- descriptors over tensors -----------------------------------------------------------
+def test_a_descriptor_keeps_its_tensors():
+    """Arenas and tables that nobody else holds must not be freed under the descriptor."""
+    import gc
+    import weakref
+    k = torch.zeros(2, 2, 4, 8, dtype=torch.float16)
+    v, table, lens = k.clone(), torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    refs = [weakref.ref(t) for t in (v, table, lens)]
+    kv = rb.paged_kv_from_tensors(k, v, table, lens)
+    del v, table, lens
+    gc.collect()
+    assert all(r() is not None for r in refs) and refs[0]().data_ptr() == kv.v_cache
+    del kv
+    gc.collect()
+    assert all(r() is None for r in refs)
