@@ -433,7 +433,9 @@ int tmllm_batch_tables(const tmllm_paged_kv* kv, const int32_t* new_lens,
  *             elements it holds.
  *   rope_cos / rope_sin  [rope_len, head_dim / 2] F32, both NULL = no rotation
  *   q_out     [rows, q_heads, head_dim] rotated queries (may be q itself, with its stride)
- *   k_out     [rows, num_kv_heads, head_dim] rotated keys (may be k itself), or NULL */
+ *   k_out     [rows, num_kv_heads, head_dim] rotated keys (may be k itself), or NULL
+ * q_out and k_out may overlap nothing else; q, k and v may lie in the arenas where the call caches
+ * nothing. */
 int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, const void* v,
                       int64_t rows, int32_t q_heads, int64_t q_stride, int64_t kv_stride,
                       const int32_t* positions, const int64_t* slots, const float* rope_cos,
@@ -452,7 +454,8 @@ int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, co
  *   scale    <= 0 means 1/sqrt(head_dim)
  *   out      [rows, q_heads, head_dim] packed (dtype, or F32 if out_f32); may be q itself
  *     (same type and stride), and must not overlap k or v
- *   lse      [rows, q_heads] F32 natural-log sums of the scaled logits (NULL ok)
+ *   lse      [rows, q_heads] F32 natural-log sums of the scaled logits (NULL ok); out and lse may
+ *     overlap nothing else
  * Keys and values behind a row do not reach its result, whatever they hold.  A value that is
  * not finite makes its element of every row that sees it non-finite: as itself, or as NaN (0 * inf)
  * where its weight rounds to zero.  A row whose logits are all -inf gives zeros and lse -inf, over

@@ -413,6 +413,28 @@ int tmllm_batch_tables(const tmllm_paged_kv* kv, const int32_t* new_lens,
         return fail(TMLLM_INVALID_ARGUMENT, "null tensor pointer");
     if (free_start && free_start >= info && free_start < info + 4)
         return fail(TMLLM_INVALID_ARGUMENT, "free_start must not lie in info, which is written");
+    // every CTA reads the lengths and lists while others write: nothing written may be read, or
+    // written as something else
+    const Span table{kv->block_table, int64_t{4} * kv->num_seqs * kv->max_blocks_per_seq};
+    const Span out[6] = {{q_start, int64_t{4} * (kv->num_seqs + int64_t{1})},
+                         {positions, 4 * rows},
+                         {row_seq, 4 * rows},
+                         {slots, 8 * rows},
+                         {info, 16},
+                         free_blocks ? table : Span{nullptr, 0}};
+    const Span in[5] = {{kv->seq_lens, int64_t{4} * kv->num_seqs},
+                        {new_lens, int64_t{4} * kv->num_seqs},
+                        {free_blocks, int64_t{4} * num_free},
+                        {free_start, 4},
+                        free_blocks ? Span{nullptr, 0} : table};
+    for (int o = 0; o < 6; ++o) {
+        for (const Span& i : in)
+            if (overlaps(out[o], i))
+                return fail(TMLLM_INVALID_ARGUMENT, "an output overlaps an input");
+        for (int p = 0; p < o; ++p)
+            if (overlaps(out[o], out[p]))
+                return fail(TMLLM_INVALID_ARGUMENT, "two outputs overlap");
+    }
     TableArgs a{};
     a.block_table = const_cast<int32_t*>(kv->block_table);  // written only with free_blocks
     a.seq_lens = kv->seq_lens;
@@ -466,12 +488,15 @@ int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, co
     if (!kv_stride) kv_stride = kw;
     if (!q_out_stride) q_out_stride = qw;
     if (!k_out_stride) k_out_stride = kw;
-    int64_t span, arena_slots;
-    if (q_stride < qw || q_out_stride < qw || kv_stride < kw || k_out_stride < kw ||
-        !mul_ok(rows, q_stride, &span) || !mul_ok(rows, kv_stride, &span) ||
-        !mul_ok(rows, q_out_stride, &span) || !mul_ok(rows, k_out_stride, &span) ||
-        span > INT64_MAX / 8 || !mul_ok(kv->num_blocks, kv->block_size, &arena_slots))
+    int64_t span, arena_slots, arena;
+    if (q_stride < qw || q_out_stride < qw || kv_stride < kw || k_out_stride < kw)
         return fail(TMLLM_INVALID_SHAPE, "row strides must cover a row");
+    for (int64_t stride : {q_stride, kv_stride, q_out_stride, k_out_stride})
+        if (!mul_ok(rows, stride, &span) || span > INT64_MAX / 8)
+            return fail(TMLLM_INVALID_SHAPE, "rows and row strides must fit 60 bits");
+    if (!mul_ok(kv->num_blocks, kv->block_size, &arena_slots) || !mul_ok(arena_slots, kw, &arena) ||
+        arena > INT64_MAX / 8)
+        return fail(TMLLM_INVALID_SHAPE, "the arenas must fit 60 bits");
     if (!q || !k || !v || !q_out || !kv->k_cache || !kv->v_cache || !positions || !slots)
         return fail(TMLLM_INVALID_ARGUMENT, "null tensor pointer");
     if ((rope_cos == nullptr) != (rope_sin == nullptr) || (rope_cos && rope_len <= 0))
@@ -496,6 +521,26 @@ int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, co
         }
     if (k_out && overlaps(out[0], out[1], rows, es))
         return fail(TMLLM_INVALID_ARGUMENT, "q_out and k_out overlap");
+    // nor may anything written be cache for the one and row, index or table for the other
+    const int64_t table = rope_cos ? int64_t{2} * rope_len * D : 0;
+    const Span arenas[2] = {{kv->k_cache, arena * static_cast<int64_t>(es)},
+                            {kv->v_cache, arena * static_cast<int64_t>(es)}};
+    const Span read[4] = {{positions, 4 * rows}, {slots, 8 * rows}, {rope_cos, table},
+                          {rope_sin, table}};
+    for (const Rows& o : out) {
+        for (const Span& c : arenas)
+            if (inside(c.p, c.bytes, o, rows, es))
+                return fail(TMLLM_INVALID_ARGUMENT, "q_out / k_out overlap the cache");
+        for (const Span& r : read)
+            if (inside(r.p, r.bytes, o, rows, es))
+                return fail(TMLLM_INVALID_ARGUMENT,
+                            "q_out / k_out overlap the positions, slots or RoPE tables");
+    }
+    for (const Span& c : arenas)
+        for (const Span& r : read)
+            if (overlaps(c, r))
+                return fail(TMLLM_INVALID_ARGUMENT,
+                            "the cache overlaps the positions, slots or RoPE tables");
     AppendArgs a{};
     a.q = q;
     a.k = k;

@@ -68,6 +68,27 @@ inline bool overlaps(const Rows& a, const Rows& b, int64_t rows, size_t es) {
     return true;
 }
 
+// Whether `bytes` bytes at p (null: none) lie in one of the rows.
+inline bool inside(const void* p, int64_t bytes, const Rows& a, int64_t rows, size_t es) {
+    if (!p || !a.p || bytes <= 0 || rows <= 0) return false;
+    const int64_t pitch = a.stride * static_cast<int64_t>(es);
+    const int64_t width = a.width * static_cast<int64_t>(es);
+    const int64_t lo = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)) -
+                       static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.p));
+    if (lo + bytes <= 0 || lo >= (rows - 1) * pitch + width) return false;
+    if (lo < 0) return true;
+    const int64_t r = rows > 1 ? lo / pitch : 0;
+    return lo - r * pitch < width || (r + 1 < rows && lo + bytes > (r + 1) * pitch);
+}
+// Whether two stretches of memory share a byte.
+struct Span {
+    const void* p;  // null: none
+    int64_t bytes;
+};
+inline bool overlaps(const Span& a, const Span& b) {
+    return inside(a.p, a.bytes, {b.p, b.bytes, b.bytes}, b.bytes > 0 ? 1 : 0, 1);
+}
+
 // Cross-GPU exchange of a sequence split (device-resident; see exchange.cu).  Every rank
 // owns one buffer of 8-byte cells {F32 value bits, step number}:
 //   recv_o   [2 parities][world][rows][head_dim]   normalised partial outputs

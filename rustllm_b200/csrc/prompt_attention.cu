@@ -1283,9 +1283,11 @@ int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, c
     if (!q_stride) q_stride = qw;
     if (!kv_stride) kv_stride = kw;
     int64_t span;
-    if (q_stride < qw || kv_stride < kw || !mul_ok(rows, q_stride, &span) ||
-        !mul_ok(rows, kv_stride, &span) || span > INT64_MAX / 8)
+    if (q_stride < qw || kv_stride < kw)
         return fail(TMLLM_INVALID_SHAPE, "row strides of q / k / v must cover a row");
+    for (int64_t stride : {q_stride, kv_stride})
+        if (!mul_ok(rows, stride, &span) || span > INT64_MAX / 8)
+            return fail(TMLLM_INVALID_SHAPE, "rows and row strides must fit 60 bits");
     if (!q || !k || !v || !q_start || !out)
         return fail(TMLLM_INVALID_ARGUMENT, "null tensor pointer");
     const size_t es = dtype_size(dtype);
@@ -1307,6 +1309,12 @@ int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, c
     }
     if (overlaps(ro, {k, kv_stride, kw}, rows, es) || overlaps(ro, {v, kv_stride, kw}, rows, es))
         return fail(TMLLM_INVALID_ARGUMENT, "out overlaps k or v");
+    const Span sums{lse, 4 * rows * q_heads}, starts{q_start, 4 * (int64_t{1} + num_seqs)};
+    for (const Rows& r : {Rows{q, q_stride, qw}, Rows{k, kv_stride, kw}, Rows{v, kv_stride, kw}, ro})
+        if (inside(sums.p, sums.bytes, r, rows, es))
+            return fail(TMLLM_INVALID_ARGUMENT, "lse overlaps q, k, v or out");
+    if (inside(starts.p, starts.bytes, ro, rows, es) || overlaps(starts, sums))
+        return fail(TMLLM_INVALID_ARGUMENT, "out or lse overlaps q_start");
     PromptArgs a{};
     a.q = q;
     a.k = k;

@@ -591,6 +591,8 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     const uintptr_t o1 = o0 + 2 * static_cast<uintptr_t>((rows - 1) * ldo + n);
     const uintptr_t w1 = w0 + 2 * static_cast<uintptr_t>((k - 1) * ldw + wide);
     if (o0 < w1 && w0 < o1) return fail(TMLLM_INVALID_ARGUMENT, "out overlaps W");
+    if (inside(bias, 2 * wide, {out, ldo, n}, rows, 2))
+        return fail(TMLLM_INVALID_ARGUMENT, "out overlaps the bias");
     LinArgs a{};
     a.bias = static_cast<const __half*>(bias);
     a.residual = static_cast<const __half*>(residual);

@@ -10,6 +10,7 @@ import torch
 import rustllm_b200 as rb
 from conftest import ROOT
 from rustllm_b200 import _lib
+from test_prompt_args import COS, K, O, POS, Q, SIN, SLOT, V, append, attention, lin, tables
 
 
 def source(name: str) -> str:
@@ -80,3 +81,63 @@ def test_a_descriptor_keeps_its_tensors():
     del kv
     gc.collect()
     assert all(r() is None for r in refs)
+
+
+# ---- what is written overlaps nothing else ----------------------------------------------
+INVALID_ARGUMENT = 1
+MB = 1 << 20
+
+
+def refused(got: int, words: bytes) -> bool:
+    return got == INVALID_ARGUMENT and words in _lib.load().tmllm_last_error()
+
+
+@pytest.mark.parametrize("lse", [Q, Q + 64, K + 4, V + 128, O, O + 8 * 256 * 2 - 4, POS, O - 4])
+def test_prompt_attention_lse_overlaps_nothing(lse):
+    """8 rows of 4 query and 2 key heads of 64; lse has 128 bytes."""
+    assert refused(attention(lse=lse), b"lse")
+
+
+def test_prompt_attention_out_overlaps_no_starts():
+    assert refused(attention(start=O + 16), b"q_start")
+    assert refused(attention(start=O - 8), b"q_start")
+
+
+def test_prompt_attention_lse_between_strided_rows_is_no_overlap():
+    """Rows of q further apart (8192 bytes) than they are wide (512): lse may lie in a gap."""
+    assert refused(attention(qs=4096, lse=Q + 512 - 4), b"lse")
+    assert refused(attention(qs=4096, lse=Q + 8192 - 124), b"lse")  # reaches row 1
+    assert refused(attention(qs=4096, lse=Q + 512, start=O), b"q_start")  # past that check
+
+
+@pytest.mark.parametrize("bias,kw", [(O, {}), (O + 2, {}), (O - 254, {}), (O + 3 * 256 + 254, {}),
+                                     (O + 1024, dict(ldo=512)), (O + 1024 - 2, dict(ldo=512))])
+def test_prompt_linear_bias_lies_outside_out(bias, kw):
+    """4 rows of 128 columns: 256 bytes a row, 1024 apart in the strided cases."""
+    assert refused(lin(bias=bias, **kw), b"bias")
+
+
+@pytest.mark.parametrize("kw", [
+    dict(qo=20 * MB), dict(qo=20 * MB + 8 * 2 * 16 * 64 * 2 - 16), dict(qo=21 * MB - 16),
+    dict(ko=21 * MB + 64), dict(qo=POS, pos=POS), dict(ko=SLOT - 16), dict(qo=COS), dict(ko=SIN),
+    dict(pos=20 * MB + 4), dict(slots=21 * MB), dict(cos=20 * MB), dict(sin=21 * MB + 128)])
+def test_rope_append_outputs_lie_apart(kw):
+    assert append(**kw) == INVALID_ARGUMENT
+    assert b"overlap" in _lib.load().tmllm_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(new=3 * MB + 4), dict(q_start=23 * MB), dict(pos=23 * MB + 4), dict(seq=2 * MB + 12),
+    dict(slots=MB), dict(info=2 * MB), dict(pos=3 * MB + 8), dict(seq=4 * MB + 28),
+    dict(slots=5 * MB - 60), dict(info=6 * MB), dict(q_start=22 * MB), dict(free=22 * MB),
+    dict(start=4 * MB), dict(pos=22 * MB + 28, free=None), dict(q_start=22 * MB + 16, free=None)])
+def test_batch_tables_outputs_lie_apart(kw):
+    assert tables(**kw) == INVALID_ARGUMENT
+    assert b"overlap" in _lib.load().tmllm_last_error()
+
+
+def test_batch_tables_empty_parts_overlap_nothing():
+    """No rows and an empty free list have no bytes (only the null length is refused here)."""
+    assert tables(rows=0, pos=3 * MB, seq=3 * MB, slots=3 * MB, free=7 * MB, num_free=0,
+                  new=None) == INVALID_ARGUMENT
+    assert b"null" in _lib.load().tmllm_last_error()
