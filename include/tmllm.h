@@ -400,11 +400,12 @@ int tmllm_prefill_status(int32_t* status);
  *               (the arenas are not touched and may be NULL)
  *   new_lens    device int32 [num_seqs]; a negative length counts as 0
  *   free_blocks device int32 [num_free] free block ids (num_free 0 with a non-NULL pointer: an
- *               empty list), or NULL: every block is already in the table.  Request s takes need_s = ceil((len + new) / bs) - ceil(len / bs) ids in
- *               request order, beginning at free_blocks[*free_start] (free_start: device int32,
- *               NULL = 0), and they are written to its block_table entries from
- *               ceil(len / bs) on.  The ids must be distinct and free; a table that
- *               tmllm_cache_* manages keeps its own list, so pass NULL for it.
+ *               empty list), or NULL: every block is already in the table.  Request s takes
+ *               need_s = ceil((len + new) / bs) - ceil(len / bs) ids in request order, beginning
+ *               at free_blocks[*free_start] (free_start: device int32, NULL = 0), and they are
+ *               written to its block_table entries from ceil(len / bs) on.  The ids must be
+ *               distinct and free.  A tmllm_cache_* hands out its own blocks: with its table a
+ *               list is refused.
  *   rows        capacity of the row arrays; rows beyond the batch get -1 in all three
  * Outputs (device): q_start int32 [num_seqs + 1]; positions int32 [rows] (len + i); row_seq
  * int32 [rows]; slots int64 [rows] (block * block_size + position % block_size, -1 without a
@@ -412,8 +413,9 @@ int tmllm_prefill_status(int32_t* status);
  * rows of the batch, requests refused, rows beyond the capacity}.
  * A request is refused - its rows get position and slot -1 and it takes no block - when its
  * cached length is negative, its tokens pass max_blocks_per_seq * block_size, or it needs
- * blocks and *free_start is negative or the needs of all requests up to it pass num_free.  Prefix sums are 64-bit and
- * saturate in the int32 outputs.  The result depends on the arguments alone: calling again
+ * blocks and *free_start is negative or the needs of all requests up to it pass num_free.
+ * Prefix sums are 64-bit and saturate in the int32 outputs.  No output may overlap an input (the
+ * table among them) or another output.  The result depends on the arguments alone: calling again
  * with the same arguments gives the same tables. */
 int tmllm_batch_tables(const tmllm_paged_kv* kv, const int32_t* new_lens,
                        const int32_t* free_blocks, int32_t num_free, const int32_t* free_start,

@@ -4,6 +4,8 @@
 #include "common.cuh"
 
 namespace tmllm {
+bool cache_owns_table(const int32_t* table);  // cache.cu
+
 namespace {
 
 // ---- block tables and slot maps ---------------------------------------------------------
@@ -413,6 +415,10 @@ int tmllm_batch_tables(const tmllm_paged_kv* kv, const int32_t* new_lens,
         return fail(TMLLM_INVALID_ARGUMENT, "null tensor pointer");
     if (free_start && free_start >= info && free_start < info + 4)
         return fail(TMLLM_INVALID_ARGUMENT, "free_start must not lie in info, which is written");
+    if (free_blocks && cache_owns_table(kv->block_table))
+        return fail(TMLLM_INVALID_ARGUMENT,
+                    "the table is a cache's, which hands out its own blocks (tmllm_cache_reserve): "
+                    "no free list");
     // every CTA reads the lengths and lists while others write: nothing written may be read, or
     // written as something else
     const Span table{kv->block_table, int64_t{4} * kv->num_seqs * kv->max_blocks_per_seq};

@@ -9,6 +9,7 @@
 // small kernels enqueued on the caller's stream, so no host buffer is read asynchronously.
 #include <algorithm>
 #include <cstring>
+#include <mutex>
 #include <random>
 #include <vector>
 
@@ -131,6 +132,7 @@ struct tmllm_cache {
     std::vector<int32_t> free_ids;  // pool, handed out from the back
     void* ws = nullptr;
     size_t ws_bytes = 0;
+    tmllm_cache* next = nullptr;  // of the list of living caches
 
     unsigned char* k_layer(int l) const { return arena + static_cast<int64_t>(2 * l) * layer_bytes; }
     unsigned char* v_layer(int l) const {
@@ -140,6 +142,23 @@ struct tmllm_cache {
 };
 
 namespace {
+
+std::mutex caches_mutex;
+tmllm_cache* caches = nullptr;
+
+void enlist(tmllm_cache* c) {
+    std::lock_guard<std::mutex> lock(caches_mutex);
+    c->next = caches;
+    caches = c;
+}
+void delist(tmllm_cache* c) {
+    std::lock_guard<std::mutex> lock(caches_mutex);
+    for (tmllm_cache** p = &caches; *p; p = &(*p)->next)
+        if (*p == c) {
+            *p = c->next;
+            return;
+        }
+}
 
 int check_cache(const tmllm_cache* c) {
     if (!c) return fail(TMLLM_INVALID_ARGUMENT, "null cache handle");
@@ -245,6 +264,15 @@ void release(tmllm_cache* c) {
 
 }  // namespace
 
+namespace tmllm {
+bool cache_owns_table(const int32_t* table) {
+    std::lock_guard<std::mutex> lock(caches_mutex);
+    for (const tmllm_cache* c = caches; c; c = c->next)
+        if (table >= c->d_table && table < c->d_table + c->h_table.size()) return true;
+    return false;
+}
+}  // namespace tmllm
+
 extern "C" {
 
 int tmllm_cache_create(const tmllm_cache_config* config, tmllm_cache** out) {
@@ -307,6 +335,7 @@ int tmllm_cache_create(const tmllm_cache_config* config, tmllm_cache** out) {
         delete c;
         return cuda_fail(e, "tmllm_cache_create allocation");
     }
+    enlist(c);
     *out = c;
     return TMLLM_OK;
 }
@@ -314,6 +343,7 @@ int tmllm_cache_create(const tmllm_cache_config* config, tmllm_cache** out) {
 int tmllm_cache_destroy(tmllm_cache* cache) {
     clear_error();
     if (!cache) return TMLLM_OK;
+    delist(cache);
     DeviceGuard guard(cache->cfg.device);
     cudaDeviceSynchronize();
     release(cache);

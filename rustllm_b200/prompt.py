@@ -118,7 +118,8 @@ def batch_tables(kv: PagedKV, new_lens: torch.Tensor, rows: int, *,
 
     ``free_blocks`` int32: ids handed out in request order, beginning at ``free_start``
     (int32 [1], default 0), and written into ``kv``'s block table; None when every block is
-    already there (a ``PagedKvCache`` view after ``reserve``).  ``rows`` is the capacity of
+    already there (a ``PagedKvCache`` view after ``reserve``: a cache hands out its own blocks, and
+    a list for its table is refused).  ``rows`` is the capacity of
     the row maps; the rest of them is -1.  Requests that do not fit are refused (their rows
     get -1, ``info[2]`` counts them)."""
     dev = new_lens.device

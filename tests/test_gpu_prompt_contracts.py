@@ -137,3 +137,31 @@ def test_prompt_attention_captured_for_shorter_prompts(cuda, dtype):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+# ---- batch_tables: the tables of a cache ------------------------------------------------
+def test_batch_tables_assigns_no_blocks_of_a_cache(cuda):
+    """A cache hands out its own blocks: ids written into its table behind its back would be given
+    to another sequence by the next reserve."""
+    cache = rb.PagedKvCache(2, 2, 64, 2, 64, num_blocks=8, device=cuda)
+    other = rb.PagedKvCache(1, 1, 64, 2, 64, device=cuda)
+    new = torch.tensor([20, 5], dtype=torch.int32, device=cuda)
+    free = torch.arange(8, dtype=torch.int32, device=cuda)
+    for layer in (0, 1):
+        with pytest.raises(rb.InvalidArgument):
+            rb.batch_tables(cache.view(layer), new, 25, free_blocks=free)
+    with pytest.raises(rb.InvalidArgument):
+        rb.batch_tables(other.view(0), new[:1], 25, free_blocks=free)
+    for s, n in enumerate((20, 5)):
+        cache.reserve(s, n)
+    m = rb.batch_tables(cache.view(0), new, 25)  # without a list: its own blocks
+    blocks = cache.block_table(0) + cache.block_table(1)
+    assert len(set(blocks)) == 3 and m.info.tolist() == [0, 25, 0, 0]
+    assert m.slots.tolist() == [blocks[i // 16] * 16 + i % 16 for i in range(20)] + \
+        [blocks[2] * 16 + i for i in range(5)]
+    # the same memory in other hands is free to be assigned again
+    view = cache.view(0)
+    table = torch.full((2, view.max_blocks_per_seq), -1, dtype=torch.int32, device=cuda)
+    view.block_table = table.data_ptr()
+    rb.batch_tables(view, new, 25, free_blocks=free)
+    assert table[:, :2].tolist() == [[0, 1], [2, -1]]
