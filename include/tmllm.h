@@ -429,7 +429,8 @@ int tmllm_batch_tables(const tmllm_paged_kv* kv, const int32_t* new_lens,
  *   q [rows, q_heads, head_dim], k, v [rows, num_kv_heads, head_dim] in the cache dtype; row
  *             strides in elements (0 = packed), so a fused QKV projection is read in place
  *   positions device int32 [rows]: a row with a negative position is padding and leaves every
- *             output as it was; a position past rope_len is not rotated
+ *             output as it was; a position from rope_len on is not rotated, and
+ *             tmllm_append_status tells
  *   slots     device int64 [rows]: block * block_size + offset; outside the arena nothing is
  *             cached for the row.  Two rows with one slot leave it unspecified which row's
  *             elements it holds.
@@ -443,6 +444,11 @@ int tmllm_rope_append(const tmllm_paged_kv* kv, const void* q, const void* k, co
                       const int32_t* positions, const int64_t* slots, const float* rope_cos,
                       const float* rope_sin, int32_t rope_len, void* q_out, int64_t q_out_stride,
                       void* k_out, int64_t k_out_stride, tmllm_stream stream);
+
+/* Reads and clears the status of tmllm_rope_append on the current device:
+ * TMLLM_POSITION_OUT_OF_RANGE when a row with a position past the rotation tables was appended
+ * (unrotated) since the last read, else TMLLM_OK.  Synchronises with the device. */
+int tmllm_append_status(int32_t* status);
 
 /* Replaces attention_core_encode (src/nn/attention.rs:216-247, start = 0) for a batch of whole
  * prompts of different lengths, packed back to back: each query row attends the rows of its

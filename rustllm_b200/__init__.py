@@ -10,8 +10,8 @@ from ._lib import (DeviceError, DeviceTimeout, InvalidArgument, InvalidDimension
 from .attention import (DecodeWorkspace, auto_splits, gqa_decode, gqa_prefill, merge_lse,
                         paged_kv_from_tensors, prefill_status)
 from .kv_cache import KvCache, LayerKvCache, PagedKvCache
-from .prompt import (BatchTables, batch_tables, prompt_attention, prompt_linear, prompt_status,
-                     rope_append)
+from .prompt import (BatchTables, append_status, batch_tables, prompt_attention, prompt_linear,
+                     prompt_status, rope_append)
 from .tensor_ops import (attention_core, attention_scale_mask, batched_matmul, concat_sequence,
                          gqa_pv_matmul, gqa_qk_matmul, kv_cache_write, repeat_kv, rope,
                          rope_tables, softmax_last_dim)
@@ -24,8 +24,8 @@ __all__ = [
     "DecodeWorkspace", "auto_splits", "gqa_decode", "gqa_prefill", "merge_lse",
     "paged_kv_from_tensors", "prefill_status",
     "KvCache", "LayerKvCache", "PagedKvCache",
-    "BatchTables", "batch_tables", "prompt_attention", "prompt_linear", "prompt_status",
-    "rope_append",
+    "BatchTables", "append_status", "batch_tables", "prompt_attention", "prompt_linear",
+    "prompt_status", "rope_append",
     "attention_core", "attention_scale_mask", "batched_matmul", "concat_sequence",
     "gqa_pv_matmul", "gqa_qk_matmul", "kv_cache_write", "repeat_kv", "rope", "rope_tables",
     "softmax_last_dim",

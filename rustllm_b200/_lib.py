@@ -216,6 +216,7 @@ _PROTOS = {
                                      vp]),
     "tmllm_rope_append": (C.c_int, [C.POINTER(PagedKV), vp, vp, vp, i64, i32, i64, i64, vp, vp, vp,
                                     vp, i32, vp, i64, vp, i64, vp]),
+    "tmllm_append_status": (C.c_int, [C.POINTER(i32)]),
     "tmllm_prompt_attention": (C.c_int, [C.c_int, vp, i64, vp, vp, i64, vp, i32, i64, i32, i32,
                                          i32, i32, C.c_float, vp, i32, vp, vp]),
     "tmllm_prompt_linear": (C.c_int, [vp, i64, vp, i64, vp, i32, vp, i64, vp, i64, i32, i32, i32,

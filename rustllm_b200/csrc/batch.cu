@@ -229,6 +229,17 @@ struct AppendArgs {
     int32_t q_heads, kv_heads, head_dim, block_size, rope_len;
 };
 
+// TMLLM_POSITION_OUT_OF_RANGE once a row's position was past the rotation tables: it is cached
+// unrotated, which no output shows.
+__device__ int g_append_status;
+
+__device__ __forceinline__ bool turned(const AppendArgs& a, int pos, bool report) {
+    if (a.cos_table == nullptr) return false;
+    if (pos < a.rope_len) return true;
+    if (report) g_append_status = TMLLM_POSITION_OUT_OF_RANGE;
+    return false;
+}
+
 // kernels/rope.metal:57-63 without contraction, F32.
 __device__ __forceinline__ void rotate(float& x1, float& x2, float c, float s) {
     const float y1 = __fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s));
@@ -257,7 +268,7 @@ __global__ void __launch_bounds__(256) rope_append_scalar_kernel(const AppendArg
                              : static_cast<const T*>(is_v ? a.v : a.k) + row * a.kv_stride) +
                        static_cast<int64_t>(h) * a.head_dim;
         T y1 = src[i], y2 = src[i + half];
-        if (!is_v && a.cos_table != nullptr && pos < a.rope_len) {
+        if (!is_v && turned(a, pos, hh == 0 && i == 0)) {
             float x1 = to_f32<T>(y1), x2 = to_f32<T>(y2);
             const int64_t e = static_cast<int64_t>(pos) * half + i;
             rotate(x1, x2, __ldg(a.cos_table + e), __ldg(a.sin_table + e));
@@ -316,7 +327,7 @@ __global__ void __launch_bounds__(256) rope_append_vec_kernel(const AppendArgs a
     }
     const int64_t head_step = static_cast<int64_t>(a.block_size) * a.head_dim;
     float cs[EPC], sn[EPC];
-    const bool turn = a.cos_table != nullptr && pos < a.rope_len;
+    const bool turn = turned(a, pos, part == 0 && lane == 0);
     if (turn) {
         const int64_t e = static_cast<int64_t>(pos) * half + c * EPC;
 #pragma unroll
@@ -393,6 +404,12 @@ int grid_of(int64_t items) {
 using namespace tmllm;
 
 extern "C" {
+
+int tmllm_append_status(int32_t* status) {
+    clear_error();
+    if (!status) return fail(TMLLM_INVALID_ARGUMENT, "null status pointer");
+    return take_status(g_append_status, status);
+}
 
 int tmllm_batch_tables(const tmllm_paged_kv* kv, const int32_t* new_lens,
                        const int32_t* free_blocks, int32_t num_free, const int32_t* free_start,

@@ -4,7 +4,8 @@
 ``rope_append`` rotates the packed q / k rows and scatters k / v into the paged cache by those
 maps, ``prompt_attention`` attends whole packed prompts causally, and ``prompt_linear`` is the
 projection of any number of rows with bias, activation and residual in its epilogue.
-``Decoder.prefill_packed`` runs a model on them.  Nothing here synchronises with the device.
+``Decoder.prefill_packed`` runs a model on them.  The four calls do not synchronise with the
+device; ``prompt_status`` and ``append_status`` do.
 """
 from __future__ import annotations
 
@@ -52,9 +53,18 @@ def _on(device: torch.device, *ts) -> None:
 
 def prompt_status() -> int:
     """Reads and clears the wait status of ``prompt_attention`` and ``prompt_linear`` on the
-    current device (0, or the TMLLM_TIMEOUT code)."""
+    current device (synchronises): 0, or the TMLLM_TIMEOUT code."""
     st = C.c_int32()
     call("tmllm_prompt_status", C.byref(st))
+    return st.value
+
+
+def append_status() -> int:
+    """Reads and clears the status of ``rope_append`` on the current device (synchronises): 0, or
+    ``PositionOutOfRange.status`` when a row with a position past the rotation tables was appended,
+    unrotated, since the last read."""
+    st = C.c_int32()
+    call("tmllm_append_status", C.byref(st))
     return st.value
 
 
@@ -164,7 +174,8 @@ def rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     q [rows, Hq, D], k, v [rows, Hkv, D] in the cache dtype (views into a fused projection are
     read in place); ``positions`` int32 [rows] and ``slots`` int64 [rows] from
-    ``batch_tables``; ``rope`` the (cos, sin) F32 tables, or None for no rotation.  Rotated
+    ``batch_tables``; ``rope`` the (cos, sin) F32 tables, or None for no rotation (a row whose
+    position is past the tables is not rotated, and ``append_status`` tells).  Rotated
     queries go to ``q_out`` (default: a new tensor, zeros in padding rows; ``q`` itself for in
     place), rotated keys and values to the cache, and the keys to ``k_out`` too when given.
     Returns (q_out, k_out)."""

@@ -165,3 +165,31 @@ def test_batch_tables_assigns_no_blocks_of_a_cache(cuda):
     view.block_table = table.data_ptr()
     rb.batch_tables(view, new, 25, free_blocks=free)
     assert table[:, :2].tolist() == [[0, 1], [2, -1]]
+
+
+# ---- rope_append: positions past the tables ---------------------------------------------
+@pytest.mark.parametrize("dtype,d", [(torch.float16, 64), (torch.float32, 128), (torch.float16, 6)])
+def test_rope_append_reports_positions_past_the_tables(cuda, dtype, d):
+    """Such rows are not rotated, which no output shows: the status does, once."""
+    g = gen(cuda, 1)
+    q, k = randn(g, 40, 4, d, dtype=dtype), randn(g, 40, 2, d, dtype=dtype)
+    c = torch.zeros(4, 2, 16, d, dtype=dtype, device=cuda)
+    kv = rb.paged_kv_from_tensors(c, c.clone(), torch.zeros((1, 4), dtype=torch.int32, device=cuda),
+                                  torch.zeros(1, dtype=torch.int32, device=cuda))
+    rope = rb.rope_tables(d, 60, 10000.0, device=cuda)
+    slots = torch.arange(40, device=cuda)
+    pos = torch.arange(20, 60, dtype=torch.int32, device=cuda)
+    rb.append_status()  # whatever ran before
+    rb.rope_append(kv, q, k, k, pos, slots, rope=rope)
+    pos[3] = -5  # padding
+    rb.rope_append(kv, q, k, k, pos, slots, rope=rope)
+    rb.rope_append(kv, q, k, k, pos + 1, slots)  # no rotation asked for
+    assert rb.append_status() == 0
+    side = torch.cuda.Stream(cuda)
+    pos[39] = 60
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        rb.rope_append(kv, q, k, k, pos, slots, rope=rope)
+    assert rb.append_status() == rb.PositionOutOfRange.status
+    assert rb.append_status() == 0
+    assert rb.prompt_status() == 0  # that is the status of the bounded waits

@@ -141,3 +141,7 @@ def test_batch_tables_empty_parts_overlap_nothing():
     assert tables(rows=0, pos=3 * MB, seq=3 * MB, slots=3 * MB, free=7 * MB, num_free=0,
                   new=None) == INVALID_ARGUMENT
     assert b"null" in _lib.load().tmllm_last_error()
+
+
+def test_append_status_refuses_null():
+    assert _lib.load().tmllm_append_status(None) == INVALID_ARGUMENT
