@@ -489,6 +489,12 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
                         int32_t activation, const void* residual, int64_t ldr, void* out,
                         int64_t ldo, int32_t rows, int32_t k, int32_t n, tmllm_stream stream);
 
+/* Which kernel tmllm_prompt_linear takes for a product on a GPU of `sms` multiprocessors (0: the
+ * current device's): form[0] accumulator columns of a tile (SwiGLU: gate and up together), form[1]
+ * CTAs that share a tile of twice the rows (1 or 2), form[2] CTAs that share its K (1, 2, 4, 8). */
+int tmllm_prompt_linear_form(int32_t rows, int32_t k, int32_t n, int32_t activation, int32_t sms,
+                             int32_t* form);
+
 /* Reads and clears the status of the bounded device-side waits in tmllm_prompt_attention and
  * tmllm_prompt_linear on the current device: TMLLM_TIMEOUT when one expired since the last
  * read (that call's outputs are undefined), else TMLLM_OK.  Synchronises with the device. */

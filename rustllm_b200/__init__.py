@@ -11,7 +11,7 @@ from .attention import (DecodeWorkspace, auto_splits, gqa_decode, gqa_prefill, m
                         paged_kv_from_tensors, prefill_status)
 from .kv_cache import KvCache, LayerKvCache, PagedKvCache
 from .prompt import (BatchTables, append_status, batch_tables, prompt_attention, prompt_linear,
-                     prompt_status, rope_append)
+                     prompt_linear_form, prompt_status, rope_append)
 from .tensor_ops import (attention_core, attention_scale_mask, batched_matmul, concat_sequence,
                          gqa_pv_matmul, gqa_qk_matmul, kv_cache_write, repeat_kv, rope,
                          rope_tables, softmax_last_dim)
@@ -25,7 +25,7 @@ __all__ = [
     "paged_kv_from_tensors", "prefill_status",
     "KvCache", "LayerKvCache", "PagedKvCache",
     "BatchTables", "append_status", "batch_tables", "prompt_attention", "prompt_linear",
-    "prompt_status", "rope_append",
+    "prompt_linear_form", "prompt_status", "rope_append",
     "attention_core", "attention_scale_mask", "batched_matmul", "concat_sequence",
     "gqa_pv_matmul", "gqa_qk_matmul", "kv_cache_write", "repeat_kv", "rope", "rope_tables",
     "softmax_last_dim",

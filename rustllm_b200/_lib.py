@@ -221,6 +221,7 @@ _PROTOS = {
                                          i32, i32, C.c_float, vp, i32, vp, vp]),
     "tmllm_prompt_linear": (C.c_int, [vp, i64, vp, i64, vp, i32, vp, i64, vp, i64, i32, i32, i32,
                                       vp]),
+    "tmllm_prompt_linear_form": (C.c_int, [i32, i32, i32, i32, i32, C.POINTER(i32)]),
     "tmllm_prompt_status": (C.c_int, [C.POINTER(i32)]),
     "tmllm_merge_lse": (C.c_int, [vp, vp, i32, i32, i32, i64, i64, vp, i32, vp, vp]),
     "tmllm_exchange_create": (C.c_int, [i32, i32, i32, i32, i32, C.POINTER(vp), vp]),

@@ -14,8 +14,8 @@
 // F16 x [rows, k], W [k, n] row-major (nn/linear.rs:26-27), F32 accumulation and F32 all the
 // way through bias, activation (kernels/silu.metal:38-46 for SwiGLU) and residual, one
 // rounding to F16 at the store.
-#include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc.cuh"
@@ -494,6 +494,57 @@ inline int64_t time_of(int64_t m_tiles, int64_t n_tiles, int units, int weight, 
     return (m_tiles * n_tiles + units - 1) / units * (weight * ksteps + 1500);
 }
 
+// Which kernel takes a product: accumulator columns of a tile, CTAs that share one (a pair or one),
+// CTAs that share its K.
+struct Form {
+    int columns, ctas, split;
+    bool gated;
+};
+
+// The fastest tile by that model: few or ragged tiles take narrow ones, large products a pair of CTAs
+// (8191 x 4096 x 4096: 190 us against 218 alone, back to back under the power limit).  Few tiles with
+// a long K: the split of K over a cluster with the shortest time, if that is shorter.  Handing the
+// sums round costs 6 units a column and CTA, and the first 6 to 8 K steps of a CTA are in flight
+// together, so shorter parts gain nothing (33 x 4096 x 512: 17.4 us in one part, 10.8, 7.9, 6.5 in
+// 2, 4, 8; 33 x 512 x 512: 4.8 in one, 5.3 in 2).
+inline Form choose(int64_t rows, int64_t k, int64_t n, bool gated, int sms) {
+    const int64_t mt = (rows + kM - 1) / kM, mp = (rows + 2 * kM - 1) / (2 * kM);
+    const int64_t ksteps = (k + 15) / 16;
+    // output columns of a tile: half of a gated one's are gate columns
+    auto tiles = [&](int columns) {
+        const int on = gated ? columns / 2 : columns;
+        return (n + on - 1) / on;
+    };
+    struct Tile {
+        int columns, weight, max_split;
+    };
+    constexpr Tile kTiles[4] = {{64, 130, 8}, {128, 170, 8}, {192, 210, 2}, {256, 256, 2}};
+    Form best{};
+    int64_t time = INT64_MAX;
+    auto offer = [&](int64_t t, int columns, int ctas, int split) {
+        if (t < time) time = t, best = {columns, ctas, split, gated};
+    };
+    for (const Tile& c : kTiles) {
+        if (gated && (c.columns == 64 || c.columns == 192)) continue;
+        offer(time_of(mt, tiles(c.columns), sms, c.weight, ksteps), c.columns, 1, 1);
+    }
+    offer(time_of(mp, tiles(256), sms / 2, 224, ksteps), 256, 2, 1);
+    for (const Tile& c : kTiles) {
+        if (gated && (c.columns == 64 || c.columns == 192)) continue;
+        for (int split = 2; split <= c.max_split; split *= 2) {
+            // 148 SMs hold 74 clusters of 2, 33 of 4, 15 of 8 at once
+            const int64_t held = split == 2 ? 74 : split == 4 ? 33 : 15;
+            if (mt * tiles(c.columns) * 148 > sms * held ||
+                (k + kK - 1) / kK < (c.columns == 64 ? 6 : 8) * split)
+                continue;
+            offer(time_of(1, 1, 1, c.weight, (ksteps + split - 1) / split) + 400 +
+                      int64_t{6} * c.columns * (split - 1),
+                  c.columns, 1, split);
+        }
+    }
+    return best;
+}
+
 template <int BN, bool GATED, bool PAIR = false, int SPLIT = 1>
 int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ldo,
            LinArgs a, cudaStream_t s) {
@@ -604,82 +655,60 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     a.n = n;
     a.act = activation;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    // the fastest tile by that model: few or ragged tiles take narrow ones, large products a pair
-    // of CTAs (8191 x 4096 x 4096: 190 us against 218 alone, back to back under the power limit)
-    const int64_t mt = (rows + kM - 1) / kM, mp = (rows + 2 * kM - 1) / (2 * kM);
-    const int64_t ksteps = (k + 15) / 16;
-    const int sms = device_sm_count();
-    auto tiles = [&](int on) { return (static_cast<int64_t>(n) + on - 1) / on; };
-    // Few tiles with a long K: the split of K over a cluster with the shortest time, if that is
-    // shorter.  Handing the sums round costs 6 units a column and CTA, and the first 6 to 8 K steps
-    // of a CTA are in flight together, so shorter parts gain nothing (33 x 4096 x 512: 17.4 us in
-    // one part, 10.8, 7.9, 6.5 in 2, 4, 8; 33 x 512 x 512: 4.8 in one, 5.3 in 2).
-    auto split_time = [&](int on, int bn, int weight, int split) {
-        const int64_t count = mt * tiles(on);
-        // 148 SMs hold 74 clusters of 2, 33 of 4, 15 of 8 at once
-        if (count * 148 > sms * (split == 2 ? 74 : split == 4 ? 33 : 15) ||
-            (k + kK - 1) / kK < (bn == 64 ? 6 : 8) * split)
-            return INT64_MAX;
-        return time_of(1, 1, 1, weight, (ksteps + split - 1) / split) + 400 +
-               int64_t{6} * bn * (split - 1);
+    const Form f = choose(rows, k, n, activation == ACT_SWIGLU, device_sm_count());
+    auto go = [&](auto bn, auto gated, auto pair, auto split) {
+        return launch<bn(), gated(), pair(), split()>(x, ldx, w, ldw, out, ldo, a, s);
     };
-    struct Split {
-        int64_t time;
-        int which;
-    } sp{INT64_MAX, 0};
-    auto offer = [&](int64_t time, int which) {
-        if (time < sp.time) sp = {time, which};
-    };
-    if (activation == ACT_SWIGLU) {
-        for (int i = 2; i <= 8; i *= 2) offer(split_time(64, 128, 170, i), i);
-        offer(split_time(128, 256, 256, 2), 1);
-    } else {
-        for (int i = 2; i <= 8; i *= 2) offer(split_time(64, 64, 130, i), i);
-        for (int i = 2; i <= 8; i *= 2) offer(split_time(128, 128, 170, i), 16 + i);
-        offer(split_time(192, 192, 210, 2), 0);
-        offer(split_time(256, 256, 256, 2), 1);
-    }
-    auto launch_split = [&]() {
-        switch (activation == ACT_SWIGLU ? 32 + sp.which : sp.which) {
-            case 0: return launch<192, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
-            case 1: return launch<256, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
-            case 2: return launch<64, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
-            case 4: return launch<64, false, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
-            case 8: return launch<64, false, false, 8>(x, ldx, w, ldw, out, ldo, a, s);
-            case 18: return launch<128, false, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
-            case 20: return launch<128, false, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
-            case 24: return launch<128, false, false, 8>(x, ldx, w, ldw, out, ldo, a, s);
-            case 33: return launch<256, true, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
-            case 34: return launch<128, true, false, 2>(x, ldx, w, ldw, out, ldo, a, s);
-            case 36: return launch<128, true, false, 4>(x, ldx, w, ldw, out, ldo, a, s);
-            default: return launch<128, true, false, 8>(x, ldx, w, ldw, out, ldo, a, s);
+    std::integral_constant<int, 64> c64;
+    std::integral_constant<int, 128> c128;
+    std::integral_constant<int, 192> c192;
+    std::integral_constant<int, 256> c256;
+    std::integral_constant<int, 1> s1;
+    std::integral_constant<int, 2> s2;
+    std::integral_constant<int, 4> s4;
+    std::integral_constant<int, 8> s8;
+    std::true_type yes;
+    std::false_type no;
+    if (f.gated) {
+        if (f.ctas == 2) return go(c256, yes, yes, s1);
+        if (f.columns == 256) return f.split == 1 ? go(c256, yes, no, s1) : go(c256, yes, no, s2);
+        switch (f.split) {
+            case 1: return go(c128, yes, no, s1);
+            case 2: return go(c128, yes, no, s2);
+            case 4: return go(c128, yes, no, s4);
+            default: return go(c128, yes, no, s8);
         }
-    };
-    if (activation == ACT_SWIGLU) {
-        const int64_t t256 = time_of(mt, tiles(128), sms, 256, ksteps);
-        const int64_t t128 = time_of(mt, tiles(64), sms, 170, ksteps);
-        const int64_t pair = time_of(mp, tiles(128), sms / 2, 224, ksteps);
-        if (sp.time < std::min(std::min(pair, t256), t128)) return launch_split();
-        if (pair < t256 && pair < t128)
-            return launch<256, true, true>(x, ldx, w, ldw, out, ldo, a, s);
-        return t256 <= t128 ? launch<256, true>(x, ldx, w, ldw, out, ldo, a, s)
-                            : launch<128, true>(x, ldx, w, ldw, out, ldo, a, s);
     }
-    const int64_t times[5] = {
-        time_of(mt, tiles(64), sms, 130, ksteps), time_of(mt, tiles(128), sms, 170, ksteps),
-        time_of(mt, tiles(192), sms, 210, ksteps), time_of(mt, tiles(256), sms, 256, ksteps),
-        time_of(mp, tiles(256), sms / 2, 224, ksteps)};
-    int best = 0;
-    for (int i = 1; i < 5; ++i)
-        if (times[i] < times[best]) best = i;
-    if (sp.time < times[best]) return launch_split();
-    switch (best) {
-        case 0: return launch<64, false>(x, ldx, w, ldw, out, ldo, a, s);
-        case 1: return launch<128, false>(x, ldx, w, ldw, out, ldo, a, s);
-        case 2: return launch<192, false>(x, ldx, w, ldw, out, ldo, a, s);
-        case 3: return launch<256, false>(x, ldx, w, ldw, out, ldo, a, s);
-        default: return launch<256, false, true>(x, ldx, w, ldw, out, ldo, a, s);
+    if (f.ctas == 2) return go(c256, no, yes, s1);
+    if (f.columns == 256) return f.split == 1 ? go(c256, no, no, s1) : go(c256, no, no, s2);
+    if (f.columns == 192) return f.split == 1 ? go(c192, no, no, s1) : go(c192, no, no, s2);
+    if (f.columns == 128) switch (f.split) {
+            case 1: return go(c128, no, no, s1);
+            case 2: return go(c128, no, no, s2);
+            case 4: return go(c128, no, no, s4);
+            default: return go(c128, no, no, s8);
+        }
+    switch (f.split) {
+        case 1: return go(c64, no, no, s1);
+        case 2: return go(c64, no, no, s2);
+        case 4: return go(c64, no, no, s4);
+        default: return go(c64, no, no, s8);
     }
+}
+
+int tmllm_prompt_linear_form(int32_t rows, int32_t k, int32_t n, int32_t activation, int32_t sms,
+                             int32_t* form) {
+    clear_error();
+    if (!form) return fail(TMLLM_INVALID_ARGUMENT, "null output");
+    if (rows <= 0 || k <= 0 || n <= 0 || sms < 0)
+        return fail(TMLLM_INVALID_SHAPE, "prompt_linear dimensions must be positive");
+    if (activation < ACT_NONE || activation > ACT_SWIGLU)
+        return fail(TMLLM_INVALID_ARGUMENT, "unknown activation %d", activation);
+    const Form f = choose(rows, k, n, activation == ACT_SWIGLU, sms ? sms : device_sm_count());
+    form[0] = f.columns;
+    form[1] = f.ctas;
+    form[2] = f.split;
+    return TMLLM_OK;
 }
 
 }  // extern "C"

@@ -328,3 +328,15 @@ def prompt_linear(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None
           0 if residual is None else n if one else residual.stride(0), out.data_ptr(),
           n if one else out.stride(0), rows, k, n)
     return out
+
+
+def prompt_linear_form(rows: int, k: int, n: int, activation: str = "none", *,
+                       sms: int = 0) -> tuple[int, int, int]:
+    """Which kernel ``prompt_linear`` takes (``tmllm_prompt_linear_form``): accumulator columns of a
+    tile, CTAs that share a tile, CTAs that share its K; on a GPU of ``sms`` multiprocessors (0: the
+    current device's)."""
+    if activation not in ACTIVATIONS:
+        raise _lib.InvalidArgument(f"unknown activation {activation!r}")
+    form = (C.c_int32 * 3)()
+    call("tmllm_prompt_linear_form", rows, k, n, ACTIVATIONS[activation], sms, form)
+    return tuple(form)

@@ -10,6 +10,7 @@ import torch
 
 import rustllm_b200 as rb
 from test_gpu_prompt import attention_case, gen, linear_case, randn
+from test_prompt_contracts import MANY_TILES
 
 pytestmark = pytest.mark.gpu
 
@@ -17,11 +18,10 @@ pytestmark = pytest.mark.gpu
 # ---- prompt_linear: several tiles a CTA -------------------------------------------------
 # Five tiles and more for every CTA (or pair), so that both accumulators, the ring of K steps and the
 # staging buffers are used again; ragged rows and columns.
-@pytest.mark.parametrize("rows,n,act", [
-    (95001, 56, "gelu"), (95001, 104, "silu"), (60001, 264, "none"), (1080, 25000, "relu"),
-    (385, 50000, "none"), (40003, 584, "gelu"),
-    (95001, 56, "swiglu"), (1080, 12176, "swiglu"), (60001, 136, "swiglu")])
-def test_prompt_linear_many_tiles_a_cta(cuda, rows, n, act):
+@pytest.mark.parametrize("rows,n,act,form", MANY_TILES)
+def test_prompt_linear_many_tiles_a_cta(cuda, rows, n, act, form):
+    if torch.cuda.get_device_properties(cuda).multi_processor_count == 148:
+        assert rb.prompt_linear_form(rows, 200, n, act) == form
     linear_case(cuda, rows, 200, n, act, bias=True, residual=True, seed=rows)
     linear_case(cuda, rows, 200, n, act, bias=True, seed=rows + 1, xpad=8)
     linear_case(cuda, rows, 72, n, act, residual=True, inplace=True, seed=rows + 2)

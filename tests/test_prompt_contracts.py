@@ -145,3 +145,50 @@ def test_batch_tables_empty_parts_overlap_nothing():
 
 def test_append_status_refuses_null():
     assert _lib.load().tmllm_append_status(None) == INVALID_ARGUMENT
+
+
+# ---- prompt_linear: the form each tested size takes -------------------------------------
+# (rows, n, activation) of the GPU tests with five tiles and more for every CTA (or pair), whatever K,
+# and their form: columns of a tile, CTAs that share one, CTAs that share its K
+MANY_TILES = [
+    (95001, 56, "gelu", (64, 1, 1)), (95001, 104, "silu", (128, 1, 1)),
+    (60001, 264, "none", (192, 1, 1)), (1080, 25000, "relu", (256, 1, 1)),
+    (385, 50000, "none", (256, 2, 1)), (40003, 584, "gelu", (256, 2, 1)),
+    (95001, 56, "swiglu", (128, 1, 1)), (1080, 12176, "swiglu", (256, 1, 1)),
+    (60001, 136, "swiglu", (256, 2, 1))]
+# (rows, k, n, activation) of those that share K
+SHARED_K = [
+    (512, 1024, 1024, "none", (64, 1, 2)), (33, 4040, 1000, "silu", (64, 1, 4)),
+    (33, 4096, 64, "none", (64, 1, 8)), (256, 4096, 4096, "gelu", (128, 1, 2)),
+    (33, 4096, 4096, "none", (128, 1, 4)), (33, 8192, 1016, "silu", (128, 1, 8)),
+    (300, 4096, 4088, "gelu", (192, 1, 2)), (500, 4104, 4096, "none", (256, 1, 2)),
+    (9, 2048, 2560, "swiglu", (128, 1, 2)), (33, 4096, 2048, "swiglu", (128, 1, 4)),
+    (70, 4104, 488, "swiglu", (128, 1, 8)), (300, 4096, 2040, "swiglu", (256, 1, 2))]
+
+
+def test_prompt_linear_sizes_of_the_tests_reach_every_form():
+    """A change of the rule must not leave a kernel without a test."""
+    seen = set()
+    for rows, n, act, form in MANY_TILES:
+        for k in (72, 200):
+            assert rb.prompt_linear_form(rows, k, n, act, sms=148) == form
+        columns = form[0] // 2 if act == "swiglu" else form[0]
+        tiles = -(-rows // (128 * form[1])) * -(-n // columns)
+        assert tiles >= 5 * (148 // form[1])
+        seen.add((act == "swiglu", *form))
+    for rows, k, n, act, form in SHARED_K:
+        assert rb.prompt_linear_form(rows, k, n, act, sms=148) == form
+        seen.add((act == "swiglu", *form))
+    assert len(seen) == 13 + 7  # all that tmllm_prompt_linear launches, plain and gated
+
+
+def test_prompt_linear_form_refusals():
+    with pytest.raises(rb.InvalidShape):
+        rb.prompt_linear_form(0, 64, 64, sms=148)
+    with pytest.raises(rb.InvalidShape):
+        rb.prompt_linear_form(1, 64, 64, sms=-1)
+    with pytest.raises(rb.InvalidArgument):
+        rb.prompt_linear_form(1, 64, 64, "tanh")
+    with pytest.raises(rb.InvalidShape):
+        rb.prompt_linear_form(BIG + 1, 64, 64, sms=148)
+    assert _lib.load().tmllm_prompt_linear_form(1, 64, 64, 0, 148, None) == INVALID_ARGUMENT
