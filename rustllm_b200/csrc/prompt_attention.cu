@@ -1276,7 +1276,7 @@ int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, c
     if (rows == 0 || max_rows == 0) return TMLLM_OK;
     if (max_rows > rows) max_rows = static_cast<int32_t>(rows);
     const float sc = scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(head_dim));
-    if (!std::isfinite(sc) || std::isnan(scale))
+    if (!std::isfinite(sc * kLog2e) || std::isnan(scale))  // (scores are kept as powers of two)
         return fail(TMLLM_INVALID_SHAPE, "attention scale must be positive and finite");
     const int64_t qw = static_cast<int64_t>(q_heads) * head_dim;
     const int64_t kw = static_cast<int64_t>(kv_heads) * head_dim;

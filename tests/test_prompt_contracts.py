@@ -192,3 +192,10 @@ def test_prompt_linear_form_refusals():
     with pytest.raises(rb.InvalidShape):
         rb.prompt_linear_form(BIG + 1, 64, 64, sms=148)
     assert _lib.load().tmllm_prompt_linear_form(1, 64, 64, 0, 148, None) == INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("scale", [3e38, 2.4e38])
+def test_prompt_attention_scale_that_overflows_as_a_power_of_two(scale):
+    """The kernels scale by log2(e) times as much: an infinite factor would make NaN of 0 scores."""
+    assert attention(scale=scale) == 2
+    assert b"scale" in _lib.load().tmllm_last_error()
