@@ -468,7 +468,9 @@ int tmllm_append_status(int32_t* status);
  * not finite makes its element of every row that sees it non-finite: as itself, or as NaN (0 * inf)
  * where its weight rounds to zero.  A row whose logits are all -inf gives zeros and lse -inf, over
  * any values.  F16 with head_dim a multiple of 8 up to 128
- * and 16-byte aligned rows runs on the tensor cores, everything else on the CUDA cores.  The order
+ * and 16-byte aligned rows runs on the tensor cores: there the probabilities are rounded to F16
+ * before the product with V (their sums stay F32) and every exponential is good to 2.6e-6.
+ * Everything else runs on the CUDA cores in F32 throughout.  The order
  * of a row's sums depends on rows and num_seqs, never on the run. */
 int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, const void* k,
                            const void* v, int64_t kv_stride, const int32_t* q_start,

@@ -887,6 +887,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     m = mt;
                 }
                 const bool rescale = __any_sync(FULL, grow && !fresh);
+                // P goes to F16 (the MMA's A operand has V's type): 2^-11 of each probability, as
+                // much as the output's own rounding; kept to 11 bits it lies in tensor memory at
+                // half the columns.  The sum l takes the unrounded ones and stays in F32.
                 // -inf (nothing visible yet): exp2(-inf - 0) = 0
                 const float sub = m == -INFINITY ? 0.f : -m;
                 const float2 sub2 = make_float2(sub, sub);
@@ -989,7 +992,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_arrive(bar(B::E + w));
             if (a.lse && live)
                 a.lse[static_cast<int64_t>(row) * a.q_heads + head] =
-                    ((m == -INFINITY ? 0.f : m) + __log2f(l)) * kLn2;
+                    ((m == -INFINITY ? 0.f : m) + log2f(l)) * kLn2;
             if (__any_sync(FULL, live && (none || (*odd_units & unit_bit)))) {
                 // (rows were stored by any lane: the vote and the barriers before it order that)
                 if (live)
