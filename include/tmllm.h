@@ -467,11 +467,14 @@ int tmllm_append_status(int32_t* status);
  * Keys and values behind a row do not reach its result, whatever they hold.  A value that is
  * not finite makes its element of every row that sees it non-finite: as itself, or as NaN (0 * inf)
  * where its weight rounds to zero.  A row whose logits are all -inf gives zeros and lse -inf, over
- * any values.  F16 with head_dim a multiple of 8 up to 128
- * and 16-byte aligned rows runs on the tensor cores: there the probabilities are rounded to F16
- * before the product with V (their sums stay F32) and every exponential is good to 2.6e-6.
- * Everything else runs on the CUDA cores in F32 throughout.  The order
- * of a row's sums depends on rows and num_seqs, never on the run. */
+ * any values.  F16 with head_dim a multiple of 8 up to 128 and 16-byte aligned rows runs on the
+ * tensor cores: there the probabilities are rounded to F16 before the product with V (their sums
+ * stay F32) and every exponential is good to 2.6e-6.  Everything else runs on the CUDA cores in
+ * F32 throughout.
+ * The order of a row's sums depends on which of the two forms runs and on rows and num_seqs; on the
+ * tensor cores also on where its sequence lies in the packed rows (keys are tiled on their grid), on
+ * the CUDA cores on q_heads and the GPU's multiprocessors.  So a prompt can come out with other last
+ * bits in another batch; the same call gives the same bits every time. */
 int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, const void* k,
                            const void* v, int64_t kv_stride, const int32_t* q_start,
                            int32_t num_seqs, int64_t rows, int32_t max_rows, int32_t q_heads,
@@ -485,8 +488,10 @@ int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, c
  *   4 swiglu: W is [k, 2n], gate then up columns, out = residual + silu(gate) * up;
  *   bias F16 [n] (swiglu [2n]) or NULL; residual F16 [rows, n] or NULL (may be out itself).
  * k and n multiples of 8, row strides multiples of 8 elements, x / W / residual / out 16-byte
- * aligned.  The order of the sums over k depends on rows, k and n (few rows and a long k are split),
- * never on the run. */
+ * aligned.  The order of the sums over k depends on rows, k, n, whether the activation is swiglu, and
+ * the GPU's multiprocessors (few tiles with a long k are split; tmllm_prompt_linear_form tells), so a
+ * row can come out with other last bits in another batch; the same call gives the same bits every
+ * time. */
 int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                         int32_t activation, const void* residual, int64_t ldr, void* out,
                         int64_t ldo, int32_t rows, int32_t k, int32_t n, tmllm_stream stream);

@@ -193,3 +193,22 @@ def test_rope_append_reports_positions_past_the_tables(cuda, dtype, d):
     assert rb.append_status() == rb.PositionOutOfRange.status
     assert rb.append_status() == 0
     assert rb.prompt_status() == 0  # that is the status of the bounded waits
+
+
+# ---- the order of sums ------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,d", [(torch.float16, 64), (torch.float16, 128), (torch.float16, 136),
+                                     (torch.float32, 64), (torch.float32, 128)])
+def test_prompt_attention_repeats_bit_for_bit(cuda, dtype, d):
+    """The order of a row's sums depends on the call, not on the run, nor on what other rows hold."""
+    g = gen(cuda, d)
+    lens = [300, 1, 0, 700, 129, 64]
+    rows, starts = sum(lens) + 6, [3]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    q, k, v = (randn(g, rows, h, d, dtype=dtype) for h in (6, 2, 2))
+    st = torch.tensor(starts, dtype=torch.int32, device=cuda)
+    first = [t.clone() for t in rb.prompt_attention(q, k, v, st, 700, want_lse=True)]
+    q[:3], k[-3:], v[-3:] = math.nan, math.nan, math.inf
+    for _ in range(5):
+        again = rb.prompt_attention(q, k, v, st, 700, want_lse=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
