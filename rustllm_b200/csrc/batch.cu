@@ -77,7 +77,7 @@ __device__ __forceinline__ void scan_pair(int64_t& rows, int64_t& blocks, int64_
 // offsets in shared memory.  A block the call assigns is read from the free list, not from
 // the table entry that another CTA writes.
 // Bound by its chain of dependent steps (launch, lengths, prefix sum, search, table entry, store):
-// 5.0 us a call in a graph for 64 requests of one token, 5.8 us for 512 requests of 83,929 rows
+// 5.0 us a call in a graph for 64 requests of one token, 6.0 us for 512 requests of 83,929 rows
 // (1.4 MB, 0.2 us of memory traffic).
 __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const TableArgs a) {
     __shared__ int64_t row0[kTabTile + 1];  // first row of each request of the tile
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256) rope_append_scalar_kernel(const AppendArg
 // read once a row.  kUnroll heads are loaded before the first is used.
 // Bound by memory: every element is read once and written once or twice (cache and dense):
 // 22,054 rows of 32/8 heads of 128 take 98 us, 6.1 TB/s or 93 % of the measured copy rate; 24 rows
-// of 9/3 heads of 64 2.6 us in a graph.
+// of 9/3 heads of 64 2.8 us in a graph.
 template <typename T>
 __global__ void __launch_bounds__(256) rope_append_vec_kernel(const AppendArgs a, int parts) {
     constexpr int EPC = 16 / sizeof(T), kUnroll = 4;

@@ -53,7 +53,7 @@ __device__ __forceinline__ int seq_rows(const PromptArgs& a, int s, int64_t* row
 // on).  DP: head size rounded up to 64 / 128 / 256.  Both products run on packed F32 pairs (two
 // multiply-adds an instruction) out of 16-byte shared-memory reads: 8 RT multiply-add pairs for
 // RT + 4 reads of 4 cycles each, which is what bounds it at long prompts (4096 tokens, 8 / 2 heads
-// of 128: 950 us, 36 TFLOP/s; 64 x 700 tokens, 9 / 3 heads of 64: 1080 us, 33), so few threads with
+// of 128: 928 us, 37 TFLOP/s; 64 x 700 tokens, 9 / 3 heads of 64: 1080 us, 33), so few threads with
 // many rows each; at short ones the chain of a CTA's tiles does, so a second team.  With F32 rows
 // on the 16-byte grid K and V are copied asynchronously, and a single team (DP <= 128) copies the
 // next tile while this one is computed.
@@ -391,9 +391,9 @@ int launch_fma_rows(const PromptArgs& a, cudaStream_t s) {
 }
 
 // 64 query rows a CTA read K and V half as often; 32 spread a small batch over more SMs, and two
-// teams halve its longest CTA (F32, 270 CTAs of 64 rows over 9 prompts of up to 413 tokens, heads
-// of 64: 31 us, 42 with one team of 256 threads; 2 x 500 tokens, 8 / 2 heads of 128: 46 against
-// 61; but 520 CTAs over 4096 tokens, heads of 128: 994 against 949).
+// teams halve its longest CTA (F32, 2 x 500 tokens, 8 / 2 heads of 128: 49 us against 65 with one
+// team of 256 threads; but 512 CTAs over 4096 tokens, heads of 128: 1016 against 928, and 64 x 700
+// tokens, 9 / 3 heads of 64: 1187 against 1082).
 template <typename T, int DP>
 int launch_fma(const PromptArgs& a, cudaStream_t s) {
     const bool small = (a.rows / 64 + a.num_seqs) * a.q_heads < 2 * device_sm_count();
@@ -429,8 +429,8 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 //   warp 11         scrub (below)
 // K and V arrive in tiles of 128 keys and are used in steps of KS: 64 above head size 64, where the
 // accumulators leave less tensor memory, and for short prompts, whose masked steps cost more than
-// a step's fixed part (heads of 64: 512 prompts of 300 tokens, 389 us in steps of 128 and 287 in
-// steps of 64; 16 of 2048 tokens 215 and 229), else 128.  S = Q K^T of a step sits in tensor memory;
+// a step's fixed part (9/3 heads of 64: 512 prompts of 300 tokens, 345 us in steps of 128 and 260 in
+// steps of 64; 16 of 2048 tokens 126 and 136), else 128.  S = Q K^T of a step sits in tensor memory;
 // its rows are read to registers (and the next step's S is computed over it), exponentiated, and P
 // is written to columns of its own as F16, from where it is the A operand of O += P V, so only V
 // crosses shared memory for the second product.
@@ -440,9 +440,9 @@ int launch_fma_d(const PromptArgs& a, cudaStream_t s) {
 // Bound by the softmax groups' own chain of waits, loads, maximum, exponentials and stores: a step
 // of 64 keys of two items of head size 128 takes about 1,850 cycles, of which the tensor pipe needs
 // 1,024 and the exponentials 768 of the MUFU's (1,024 without the quarter that goes to the
-// multiply-add pipe); 54 % of the issue slots are used.  16384 rows of 32/8 heads of 128: 1.71 ms,
-// 1.29 PFLOP/s; 4 x 4096 rows of 32/8 heads of 64: 368 us, 747 TFLOP/s; 64 prompts of up to 2048
-// tokens, 15/5 heads of 64: 350 us, 437 TFLOP/s.
+// multiply-add pipe); 54 % of the issue slots are used.  16384 rows of 32/8 heads of 128: 1.75 ms,
+// 1.26 PFLOP/s; 4 x 4096 rows of 32/8 heads of 64: 359 us, 766 TFLOP/s; 64 prompts of 1 to 2048
+// tokens (39,424 rows), 15/5 heads of 64: 221 us in a graph, 450 TFLOP/s.
 //
 // Masked places never reach a result: scores that a row does not see are replaced by -inf before
 // the maximum, and since 0 * inf is not 0, the non-finite entries of every V tile that some row
@@ -603,8 +603,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // reweighted to an even relative error of 2.6e-6; P is rounded to 2^-11 behind it) and 2^n put
 // together as a float.  -127 and below give 0, NaN stays.  The softmax's time is the MUFU unit's,
 // which does 4 exponentials a cycle and quarter of an SM, so every fourth pair is computed here
-// (4 x 4096 tokens, 32/8 heads of 64: 401 us without, 385 with every eighth, 382 every fourth,
-// 386 every third).
+// (4 x 4096 tokens, 32/8 heads of 64: 375 us without, 358 with every eighth, 359 every fourth,
+// 377 every third).
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
     constexpr float C0 = 0.999999285f, C1 = 0.693121791f, C2 = 0.240247443f, C3 = 0.0559178367f,
                     C4 = 0.00957007986f;
@@ -631,7 +631,8 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 __device__ __forceinline__ bool odd_half(uint32_t bits) { return (bits & 0x7C00u) == 0x7C00u; }
 
 // What a stored row lacks (rare, and out of line: the mere code of it cost instruction fetches in
-// the hot loop; 512 prompts of 300 tokens, 9/3 heads of 64: 290 us inline, 272 without).  The
+// the hot loop; 512 prompts of 300 tokens, 9/3 heads of 64: 290 us inline, 272 without, when it was
+// taken out).  The
 // non-finite values that the scrub took out of V (`vg`: column 0 of the KV head) are added to a row
 // that sees keys first .. row.  A row without a key (`none`: every score -inf) becomes zeros, since
 // the product made NaN of 0 * inf in the tiles that were not scrubbed.
@@ -1344,8 +1345,8 @@ int tmllm_prompt_attention(tmllm_dtype dtype, const void* q, int64_t q_stride, c
                     aligned16(out) && q_stride < (int64_t{1} << 38) && kv_stride < (int64_t{1} << 38);
     if (!tc) return launch_fma_d<__half>(a, s);
     if (head_dim > 64) return launch_tc<128, 64>(a, s);
-    // (see KS at the kernel; 32 prompts of 1024 tokens of 15/5 heads of 64: 138 us in steps of 128,
-    // 143 of 64; 64 of 1 to 1500 tokens 233 and 219)
+    // (see KS at the kernel; 32 prompts of 1024 tokens of 15/5 heads of 64: 130 us in steps of 128,
+    // 133 of 64; 64 of 1 to 1500 tokens 200 and 186)
     if (rows < 1024 * static_cast<int64_t>(num_seqs)) return launch_tc<64, 64>(a, s);
     return launch_tc<64, 128>(a, s);
 }

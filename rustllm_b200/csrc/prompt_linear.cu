@@ -5,11 +5,11 @@
 // A persistent grid walks the output tiles: one warp feeds x and W tiles through a ring by TMA,
 // one issues the products into one of two accumulators in tensor memory, eight empty the other
 // one, so the epilogue runs under the next tile's products.  Bound by the tensor pipe (92 % active
-// at 8191 x 4096 x 4096 with bias and residual, 179 us = 1.54 PFLOP/s at first, 229 us back to back
-// under the power limit, where a library product alone takes 235) and by latency for few rows
-// (33 x 768 x 2048: 6.4 us in a graph, 10 us a call), where K is split over the CTAs of a cluster
-// if it is long (33 x 4096 x 64: 5.9 us instead of 16.9, library product 6.7; 33 x 4096 x 4096: 12.6
-// instead of 18.5, library 9.7).
+// at 8191 x 4096 x 4096 with bias and residual, 178 us = 1.54 PFLOP/s at first, 232 us back to back
+// under the power limit, where a library product alone takes 237) and by latency for few rows
+// (33 x 768 x 2048: 6.4 us in a graph, 9.4 with bias, 10 us a call), where K is split over the CTAs
+// of a cluster if it is long (33 x 4096 x 64: 6.0 us instead of 17.2, library product 6.7; 33 x 4096
+// x 4096: 10.7 instead of 17.7, library 8.5).
 //
 // F16 x [rows, k], W [k, n] row-major (nn/linear.rs:26-27), F32 accumulation and F32 all the
 // way through bias, activation (kernels/silu.metal:38-46 for SwiGLU) and residual, one
@@ -505,8 +505,8 @@ struct Form {
 // (8191 x 4096 x 4096: 190 us against 218 alone, back to back under the power limit).  Few tiles with
 // a long K: the split of K over a cluster with the shortest time, if that is shorter.  Handing the
 // sums round costs 6 units a column and CTA, and the first 6 to 8 K steps of a CTA are in flight
-// together, so shorter parts gain nothing (33 x 4096 x 512: 17.4 us in one part, 10.8, 7.9, 6.5 in
-// 2, 4, 8; 33 x 512 x 512: 4.8 in one, 5.3 in 2).
+// together, so shorter parts gain nothing (33 x 4096 x 512: 17.3 us in one part, 10.6, 7.6, 6.2 in
+// 2, 4, 8).
 inline Form choose(int64_t rows, int64_t k, int64_t n, bool gated, int sms) {
     const int64_t mt = (rows + kM - 1) / kM, mp = (rows + 2 * kM - 1) / (2 * kM);
     const int64_t ksteps = (k + 15) / 16;

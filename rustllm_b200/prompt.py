@@ -231,7 +231,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
                      want_lse: bool = False):
     """Causal attention over whole packed prompts (``tmllm_prompt_attention``).
 
-    q [rows, Hq, D], k, v [rows, Hkv, D] (row-strided views allowed); ``q_start`` int32
+    q [rows, Hq, D], k, v [rows, Hkv, D] (row-strided views allowed, k and v with one row
+    stride); ``q_start`` int32
     [num_seqs + 1] first rows on the device; ``max_rows`` the longest sequence or about that (it
     sizes the launch; results do not depend on it, but 0 does nothing).  Row i of a sequence
     attends its rows 0 .. i.  Returns out [rows, Hq, D] in ``out_dtype`` (q's, or
