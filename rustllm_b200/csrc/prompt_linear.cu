@@ -625,9 +625,13 @@ int tmllm_prompt_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     for (int64_t ld : {ldx, ldw, ldo, ldr})
         if (ld % 8 || ld > (int64_t{1} << 38))  // the tensor maps' stride limit is 2^40 bytes
             return fail(TMLLM_INVALID_SHAPE, "row strides must be multiples of 8 elements");
-    if (ldx < k || ldw < wide || ldo < n || (residual && ldr < n) || !mul_ok(rows, ldx, &span) ||
-        !mul_ok(rows, ldo, &span) || !mul_ok(k, ldw, &span) || (residual && !mul_ok(rows, ldr, &span)))
+    if (ldx < k || ldw < wide || ldo < n || (residual && ldr < n))
         return fail(TMLLM_INVALID_SHAPE, "row strides must cover a row");
+    for (int64_t ld : {ldx, ldo, residual ? ldr : 0})
+        if (!mul_ok(rows, ld, &span) || span > INT64_MAX / 8)
+            return fail(TMLLM_INVALID_SHAPE, "rows and row strides must fit 60 bits");
+    if (!mul_ok(k, ldw, &span) || span > INT64_MAX / 8)
+        return fail(TMLLM_INVALID_SHAPE, "rows and row strides must fit 60 bits");
     for (const void* p : {x, w, residual, static_cast<const void*>(out)})
         if (!aligned16(p))
             return fail(TMLLM_INVALID_ARGUMENT, "x, w, residual and out must be 16-byte aligned");

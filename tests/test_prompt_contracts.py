@@ -199,3 +199,14 @@ def test_prompt_attention_scale_that_overflows_as_a_power_of_two(scale):
     """The kernels scale by log2(e) times as much: an infinite factor would make NaN of 0 scores."""
     assert attention(scale=scale) == 2
     assert b"scale" in _lib.load().tmllm_last_error()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: lin(rows=1 << 28, ldo=1 << 34), lambda: lin(rows=1 << 28, ldx=1 << 34),
+    lambda: lin(rows=1 << 28, res=V, ldr=1 << 34), lambda: lin(k=1 << 28, ldx=1 << 28, ldw=1 << 34),
+    lambda: attention(rows=1 << 28, qs=1 << 33), lambda: append(rows=1 << 28, qs=1 << 33),
+    lambda: append(rows=1 << 28, qos=1 << 33)])
+def test_extents_whose_bytes_overflow_are_refused(call):
+    """2^61 elements and more: their bytes do not fit the checks for overlaps."""
+    assert call() == 2
+    assert b"60 bits" in _lib.load().tmllm_last_error()
