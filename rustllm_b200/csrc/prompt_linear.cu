@@ -306,6 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto load_res = [&](int c0, int b) {
                 const int col = n * Cfg::ON + c0;
                 if (!a.residual || c0 >= Cfg::ON || col >= a.n || lane != 0) return;
+                if (*abort_flag) return;  // the buffer's last load may still be in flight
                 bulk_wait_read<0>();
                 mbar_arrive_tx(res_full(warp - 2, b), 2048);
                 sent ^= 1u << b;
